@@ -471,6 +471,59 @@ int rtg_adamw(float* params, const float* grads, float* exp_avg, float* exp_avg_
               float grad_scale, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * rtg_layernorm_* — layer norm over the axis of n elements of x = [outer][n][inner]: the last axis (inner 1: rows of
+ * activations) or the channel axis of feature maps (outer clips, n channels, inner positions).
+ *   y = (x - mean) * rstd * weight + bias,   mean / var over n,   rstd = 1 / sqrt(var + eps)
+ * x, y, dy, dx are float or bf16 (bf16 != 0), weight / bias and their gradients float or bf16 (param_bf16 != 0); every sum
+ * is held in fp32, a result is rounded once.  x may be strided: x_outer elements between slices, x_n along n (inner 1: x_n
+ * has to be 1; else positions are adjacent); y, dy, dx are contiguous [outer][n][inner].
+ * weight / bias may be NULL (1 / 0).  mean, rstd [outer * inner]: kept for the backward, both NULL without one.
+ * The variance is taken around the mean (two sums over values held in registers), so a level far from zero costs no digits.
+ * Backward:  g = dy * weight;  dx = rstd * (g - mean_n(g) - xhat * mean_n(g * xhat));  dweight = sum dy * xhat and
+ * dbias = sum dy over outer and inner, written (not added), summed in an order that only the sizes decide.  Each of dx,
+ * dweight, dbias may be NULL; ws: rtg_layernorm_ws(d) floats where dweight or dbias is given.
+ * n >= 1; outer or inner 0: nothing but zeros in dweight / dbias.
+ * ------------------------------------------------------------------------------------------------------------ */
+typedef struct RtgLayerNormDesc {
+  long long outer, n, inner, x_outer, x_n;
+  int bf16, param_bf16;
+  float eps;
+} RtgLayerNormDesc;
+int rtg_layernorm_forward(const RtgLayerNormDesc* d, const void* x, const void* weight, const void* bias, void* y,
+                          float* mean, float* rstd, void* stream);
+long long rtg_layernorm_ws(const RtgLayerNormDesc* d);
+int rtg_layernorm_backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const float* mean, const float* rstd,
+                           const void* weight, void* dx, void* dweight, void* dbias, float* ws, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * The norm over many gradient tensors, and clipping by it.  Tensor i: counts[i] adjacent elements at grads[i], float or bf16
+ * (bf16[i] != 0), any element alignment.  The three arrays are HOST memory, read during the call (they travel in the
+ * launches' arguments: legal under stream capture).  kind RTG_NORM_L2: sqrt(sum g^2), squares and sums in 64 bits (no
+ * gradient a float holds overflows or vanishes on the way); RTG_NORM_MAX: max |g|.  NaN in, NaN out.  Sums are taken in
+ * an order that the list decides: the same list gives the same bits.
+ *   rtg_grad_norm  *norm_out = norm
+ *   rtg_grad_clip  ... and g *= min(1, max_norm / (norm + 1e-6)); nothing is written where that factor is 1 (an infinite
+ *                  norm: factor 0; a NaN: NaN).  Tensors must not overlap.
+ *   rtg_adamw_clipped   the update of rtg_adamw for n flat buffers with gradients read as g * grad_scale * factor, the
+ *                  factor that of rtg_grad_clip over all n with norm * grad_scale, the 2-norm (the gradients stay as they
+ *                  are).  A buffer whose *loss_flag is NaN is left alone, its step counter included; with a norm that is
+ *                  not finite every buffer is.
+ * ws: rtg_grad_ws(n) doubles of scratch.
+ * ------------------------------------------------------------------------------------------------------------ */
+enum { RTG_NORM_L2 = 0, RTG_NORM_MAX = 1 };
+typedef struct RtgAdamWJob {
+  float* params; const float* grads; float* exp_avg; float* exp_avg_sq; float* step_state; const float* loss_flag;
+  long long n;
+} RtgAdamWJob;
+long long rtg_grad_ws(int n);
+int rtg_grad_norm(int n, const void* const* grads, const long long* counts, const int* bf16, int kind,
+                  double* ws, float* norm_out, void* stream);
+int rtg_grad_clip(int n, void* const* grads, const long long* counts, const int* bf16, int kind,
+                  double max_norm, double* ws, float* norm_out, void* stream);
+int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs_host, double max_norm, double lr, double beta1, double beta2, double eps,
+                      double weight_decay, float grad_scale, double* ws, float* norm_out, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
  * rtg_resstack_* — a whole ResidualStack (generator.py:33-77: three times r = conv_d(lrelu(x)), x = x + conv_1(lrelu(r)),
  * k = 3, d = 1, 3, 9; optional leaky-relu on the final x) in ONE launch per direction, for the stacks whose clips fit in
  * LDS: (C, L) = (128, 32) and (64, 256).  Replaces the 6 Conv1d forward and 6 backward-data launches of a stack.

@@ -1,0 +1,127 @@
+"""Layer norm, gradient norm and clipping without a GPU: the checks in front of every launch, on the Python side and at the C
+entry points, and the references that the GPU tests compare with."""
+import ctypes as C
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from norm_reference import Reference, inside
+
+
+def test_cpu_tensors_are_refused():
+    import train
+    from models.layers import LayerNorm
+    from rtg import ops
+    from rtg.lib import RtgError
+    x = torch.zeros(4, 8)
+    for call in (lambda: ops.layer_norm(x), lambda: LayerNorm(8, dim=-1)(x), lambda: LayerNorm(8)(x), lambda: ops.total_norm([x]),
+                 lambda: ops.clip_grads_([x], 1.0), lambda: ops.clipped_adamw_([x], [x], [x], [x], [x[0, :1]], 1.0)):
+        with pytest.raises(RtgError):
+            call()
+    p = torch.nn.Parameter(x)
+    p.grad = x.clone()
+    with pytest.raises(RtgError):
+        train.clip_grad_norm_([p], 1.0)
+    for bad in (-1.0, float('nan'), torch.ones(())):
+        with pytest.raises(RtgError):
+            train.AdamW([], max_norm=bad)
+    assert train.AdamW([], max_norm=2).max_norm == 2.0 and train.AdamW([]).max_norm is None
+    import hparam as hp
+    assert hp.grad_clip is None
+
+
+def test_a_banked_model_lists_its_layer_norms():
+    from models.layers import BankedModel, LayerNorm
+
+    class Net(BankedModel):
+        def __init__(self):
+            super().__init__()
+            self.norms = torch.nn.ModuleList([LayerNorm(4), LayerNorm(5, bias=False), LayerNorm(6, affine=False)])
+    net = Net()
+    names = [n for n, _ in net._extra_bank_params()]
+    assert names == ['norms.0.weight', 'norms.0.bias', 'norms.1.weight'] == [n for n, _ in net.named_parameters()]
+
+
+def test_axes_around_the_normalised_one():
+    """what the kernels read in place, and what is copied first"""
+    from rtg.ops import _axes, _norm_desc
+    t = torch.zeros(6, 40, 90)
+    assert _axes((6, 40), (3600, 90), 0, 2) == (240, 90) and _axes((6, 1, 40), (3600, 7, 90), 0, 3) == (240, 90)
+    assert _axes((6, 40), (90, 540), 0, 2) is None and _axes((), (), 0, 0) == (1, 1)
+    for x, dim, want, same in ((t, 2, (240, 90, 1, 90, 1), True), (t[:, :, 3:67], 2, (240, 64, 1, 90, 1), True),
+                               (t[:, -1], 1, (6, 90, 1, 3600, 1), True), (t[:, :, 5:44], 1, (6, 40, 39, 3600, 90), True),
+                               (t[:, 7:30], 1, (6, 23, 90, 3600, 90), True), (t, 0, (1, 6, 3600, 1, 3600), True),
+                               (t[:1, :1].expand(6, 40, 90), 2, (240, 90, 1, 0, 1), True),
+                               (t[:, :, ::2], 1, (6, 40, 45, 1800, 45), False), (t.permute(1, 0, 2), 2, (240, 90, 1, 90, 1), False),
+                               (t[:0], 2, (0, 90, 1, 0, 1), True)):
+        y, d = _norm_desc(x, None, 1e-5, dim)
+        assert (d.outer, d.n, d.inner, d.x_outer, d.x_n) == want and (y.data_ptr() == x.data_ptr()) == same, (tuple(x.shape), dim)
+
+
+def test_c_entry_points_refuse_before_any_launch():
+    from rtg.lib import AdamWJob, LayerNormDesc, lib
+    one = C.c_void_p(256)
+
+    def desc(outer=2, n=8, inner=1, x_outer=8, x_n=1, eps=1e-5):
+        return C.byref(LayerNormDesc(outer, n, inner, x_outer, x_n, 0, 0, eps))
+
+    def fwd(d, x=one, y=one, mean=None, rstd=None):
+        return lib.rtg_layernorm_forward(d, x, None, None, y, mean, rstd, None)
+    assert fwd(None) == -3 and fwd(desc(), x=None) == -3 and fwd(desc(), y=None) == -3 and fwd(desc(), mean=one) == -3
+    for bad in (desc(n=0), desc(outer=-1), desc(inner=-1), desc(x_n=2), desc(x_outer=-8), desc(eps=-1.0), desc(eps=float('nan'))):
+        assert fwd(bad) == -1 and lib.rtg_layernorm_ws(bad) == -1
+    for far in (desc(outer=1 << 40, n=1 << 30), desc(n=1 << 31), desc(outer=1 << 40, x_outer=1 << 40)):
+        assert fwd(far) == -2 and lib.rtg_layernorm_ws(far) == -2
+    assert fwd(desc(outer=0)) == 0 and lib.rtg_layernorm_ws(desc()) >= 16
+    bwd = lib.rtg_layernorm_backward
+    assert bwd(desc(), one, one, None, one, None, one, None, None, None, None) == -3
+    assert bwd(desc(), one, one, one, one, None, one, one, None, None, None) == -3           # no scratch for dweight
+    assert bwd(desc(outer=0), None, None, None, None, None, None, None, None, None, None) == 0
+
+    def arrays(ptrs, counts, bf16):
+        n = len(ptrs)
+        return n, (C.c_void_p * n)(*ptrs), (C.c_longlong * n)(*counts), (C.c_int * n)(*bf16)
+
+    def clip(lists, limit=1.0, kind=0, ws=one, out=one):
+        return lib.rtg_grad_clip(*lists, kind, limit, ws, out, None)
+    good = arrays([256, 4096], [10, 10], [0, 1])
+    assert lib.rtg_grad_norm(0, *good[1:], 0, one, one, None) == -1 and lib.rtg_grad_norm(*good, 2, one, one, None) == -1
+    assert lib.rtg_grad_norm(*good, 0, None, one, None) == -3 and lib.rtg_grad_norm(*good, 0, one, None, None) == -3
+    assert lib.rtg_grad_norm(2, None, good[2], good[3], 0, one, one, None) == -3
+    assert clip(good, limit=-1.0) == -1 and clip(good, limit=float('nan')) == -1 and clip(good, out=None) == -3
+    assert clip(arrays([256, 0], [10, 10], [0, 0])) == -3 and clip(arrays([256], [-1], [0])) == -1
+    assert clip(arrays([256], [1 << 60], [0])) == -2
+    assert clip(arrays([258], [10], [0])) == -1 and clip(arrays([257], [10], [1])) == -1     # not on an element's boundary
+    for overlap in (([256, 256], [10, 10], [0, 0]), ([256, 294], [10, 10], [0, 1]), ([4096, 256], [10, 961], [0, 0])):
+        assert clip(arrays(*overlap)) == -1
+    assert lib.rtg_grad_ws(0) == -1 and lib.rtg_grad_ws(1) >= 2049
+
+    def adamw(jobs, limit=1.0, ws=one):
+        return lib.rtg_adamw_clipped(len(jobs), (AdamWJob * max(len(jobs), 1))(*jobs), limit, 1e-3, 0.9, 0.99, 1e-8, 0.01, 1.0, ws, one, None)
+    job = (256, 512, 1024, 2048, 4096, None, 10)
+    assert adamw([]) == -1 and adamw([job], ws=None) == -3 and adamw([job], limit=-1.0) == -1
+    for i in range(5):
+        assert adamw([job[:i] + (None,) + job[i + 1:]]) == -3
+        assert adamw([job[:i] + (job[i] + 2,) + job[i + 1:]]) == -1
+    assert adamw([job[:6] + (0,)]) == -1 and adamw([job, job]) == -1 and adamw([job[:6] + (100,)]) == -1
+    assert adamw([job[:6] + (1 << 60,)]) == -2
+
+
+@pytest.mark.parametrize('kind', [torch.float32, torch.bfloat16])
+def test_the_reference_is_layer_norm_and_its_bounds_hold_for_a_float_evaluation(kind):
+    gen = torch.Generator().manual_seed(1)
+    x, dy = (torch.randn(3, 50, 7, generator=gen).to(kind) for _ in range(2))
+    w, b = torch.randn(50, generator=gen), torch.randn(50, generator=gen)
+    ref = Reference(x, w, b, 1e-5).backward(dy, torch.float32)
+    leaves = [t.double().requires_grad_(True) for t in (x, w, b)]
+    y = F.layer_norm(leaves[0].transpose(1, 2), (50,), leaves[1], leaves[2]).transpose(1, 2)
+    for got, want in zip((y, *torch.autograd.grad(y, leaves, dy.double())), (ref.y, ref.dx, ref.dw, ref.db)):
+        assert (got - want).abs().max() <= 1e-11
+    xf = x.float().transpose(1, 2)
+    yf = F.layer_norm(xf, (50,), w, b).transpose(1, 2)
+    inside(yf.to(kind), ref.y, ref.y_off, 'y')
+    # a planted mistake is outside: the variance of n - 1
+    wrong = (xf - xf.mean(2, keepdim=True)) / (xf.var(2, keepdim=True) + 1e-5).sqrt() * w + b
+    with pytest.raises(AssertionError):
+        inside(wrong.transpose(1, 2).to(torch.float32 if kind == torch.float32 else kind), ref.y, ref.y_off, 'y')

@@ -19,6 +19,11 @@ LIB = os.path.join(HERE, 'librtg.so')
 STAMP = os.path.join(HERE, 'csrc', '.build_stamp')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-comment', '-Wno-unused-result',
          '-Rpass-analysis=kernel-resource-usage'] + os.environ.get('RTG_EXTRA_FLAGS', '').split()
+# further flags of single translation units: the float loops of these bandwidth kernels must not become packed fp32
+# instructions (v_pk_*_f32: no rate is lost, the kernels wait for memory; some of their forms have been seen to give wrong
+# results on this hardware)
+_NO_PACKED_FP32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+UNIT_FLAGS = {'rtg_layernorm': _NO_PACKED_FP32, 'rtg_gradnorm': _NO_PACKED_FP32}
 # No kernel of the library may touch scratch memory (a spilled instance is a slower duplicate of a block shape that fits: round 5
 # shipped 70 of them): the compiler's per-kernel resource remarks are kept next to each object (<obj>.res), summarised by
 # kernel_resources() (tools/kernel_resources.py writes the table under profiles/), and check_no_scratch() fails the build.
@@ -38,9 +43,14 @@ def _headers_digest():
     return h
 
 
+def _unit_flags(src):
+    return UNIT_FLAGS.get(os.path.basename(src)[:-4], [])
+
+
 def _obj_digest(src, hd):
     h = hd.copy()
     h.update(open(src, 'rb').read())
+    h.update(' '.join(_unit_flags(src)).encode())
     return h.hexdigest()
 
 
@@ -151,7 +161,7 @@ def build(force=False, verbose=True):
     todo.sort(key=lambda t: -_COST.get(os.path.basename(t[0])[:-4].rstrip('0123456789'), 1))
     for s, o, st, dig in todo:
         reap(JOBS - 1)
-        cmd = [hipcc, *FLAGS, '-c', s, '-o', o]
+        cmd = [hipcc, *FLAGS, *_unit_flags(s), '-c', s, '-o', o]
         if verbose:
             print(' '.join(cmd), flush=True)
         if os.path.exists(st):

@@ -1,0 +1,456 @@
+// rtg_gradnorm.hip — the norm over many gradient tensors, clipping by it, and the AdamW update that reads clipped gradients
+// (see include/rtg.h, rtg_grad_norm / rtg_grad_clip / rtg_adamw_clipped).
+//
+//   norm = sqrt(sum_t sum_i g_t[i]^2)  or  max |g|;   factor = min(1, max_norm / (norm + 1e-6))
+//
+// One multiply-add per element of 2 or 4 bytes: bound by HBM (and, for a small model, by the launches).  The tensors are cut
+// into chunks of one size, a workgroup each, whatever their number: 172 tensors of a generator are one launch.  A chunk's sum
+// is a double: the square of any float is a normal double, so nothing overflows or vanishes, and the result does not depend
+// on how a list is cut into tensors beyond the last bits of a double.
+#include "rtg_vec.h"
+#include <algorithm>
+#include <memory>
+#include <new>
+
+namespace {
+
+constexpr int TABLE = 160;            // tensors per launch: the table travels in the kernel's arguments (3.2 KB of 4)
+constexpr int JOBS = 32;              // AdamW buffers per launch
+constexpr int BLOCKS = 2048;          // chunks a list is cut into at least, where it is long: 8 workgroups per CU
+constexpr int THREADS = 256;
+constexpr int REDUCE = 1024;
+
+struct GradTable {
+  void* p[TABLE];
+  long long n[TABLE];
+  int first[TABLE];                   // first workgroup of tensor i in this launch (increasing; empty tensors have none)
+  unsigned bf16[TABLE / 32];
+  int count;
+  long long chunk;                    // bytes of a chunk, a multiple of 4096
+};
+
+// the table's entry that workgroup b works on: the last one with first <= b.  Every lane compares its own entries (one round
+// of loads in flight together; a binary search is eight dependent ones)
+__device__ __forceinline__ int entry_of(const int* first, int count, int b) {
+  int found = 0;
+#pragma unroll
+  for (int k = 0; k < (TABLE + 63) / 64; ++k) {
+    const int i = k * 64 + (threadIdx.x & 63);
+    found += __popcll(__ballot(i < count && first[i] <= b));
+  }
+  return __builtin_amdgcn_readfirstlane(found) - 1;
+}
+
+template <int KIND>
+__device__ __forceinline__ double join(double a, double b) {
+  if constexpr (KIND == RTG_NORM_L2) return a + b;
+  return (b > a || b != b) ? b : a;                      // (a NaN stays: nothing compares greater)
+}
+template <int KIND>
+__device__ __forceinline__ double take(double acc, float v) {
+  if constexpr (KIND == RTG_NORM_L2) return fma((double)v, (double)v, acc);
+  return join<KIND>(acc, (double)fabsf(v));
+}
+
+// over the N threads of a block, result in every thread; `red`: N / 64 doubles of LDS
+template <int KIND, int N>
+__device__ __forceinline__ double block_join(double v, double* red) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = join<KIND>(v, __shfl_xor(v, off, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int i = 1; i < N / 64; ++i) v = join<KIND>(v, red[i]);
+  return v;
+}
+
+// the partials of all chunks, in an order their number decides; result in every thread
+template <int KIND, int N>
+__device__ __forceinline__ double all_partials(const double* __restrict__ part, int n, double* red) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += N) acc = join<KIND>(acc, part[i]);
+  return block_join<KIND, N>(acc, red);
+}
+
+template <int KIND>
+__device__ __forceinline__ double norm_of(double joined) { return KIND == RTG_NORM_L2 ? sqrt(joined) : joined; }
+
+// min(1, max_norm / (norm + 1e-6)): 0 for an infinite norm, NaN for a NaN
+__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
+  const double f = max_norm / (norm + 1e-6);
+  return f < 1.0 || f != f ? (float)f : 1.f;
+}
+
+template <class T, int KIND>
+__device__ __forceinline__ double chunk_sum(const T* __restrict__ p, long long n) {
+  constexpr int N = RtgVec<T>::N;
+  const long long nv = n / N;
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  long long i = threadIdx.x;
+  for (; i + 3 * THREADS < nv; i += 4 * THREADS) {
+    RtgVec<T> v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k].load(p + (i + k * THREADS) * N);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[k] = take<KIND>(acc[k], v[k].get(e));
+  }
+  for (; i < nv; i += THREADS) {
+    RtgVec<T> v;
+    v.load(p + i * N);
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[0] = take<KIND>(acc[0], v.get(e));
+  }
+  if (nv * N + threadIdx.x < n) acc[1] = take<KIND>(acc[1], rtg_up(p[nv * N + threadIdx.x]));
+  return join<KIND>(join<KIND>(acc[0], acc[1]), join<KIND>(acc[2], acc[3]));
+}
+
+// what workgroup blockIdx.x covers: [lo, lo + n) of entry i
+struct Piece { int i; long long lo, n; bool bf; };
+__device__ __forceinline__ Piece piece_of(const GradTable& t) {
+  Piece r;
+  r.i = entry_of(t.first, t.count, blockIdx.x);
+  r.bf = (t.bf16[r.i >> 5] >> (r.i & 31)) & 1;
+  const long long size = t.chunk >> (r.bf ? 1 : 2);
+  r.lo = (long long)((int)blockIdx.x - t.first[r.i]) * size;
+  const long long left = t.n[r.i] - r.lo;
+  r.n = left < size ? left : size;
+  return r;
+}
+
+template <int KIND>
+__global__ __launch_bounds__(THREADS) void grad_partial(const GradTable t, double* __restrict__ part) {
+  __shared__ double red[THREADS / 64];
+  const Piece c = piece_of(t);
+  double acc;
+  if (c.bf) acc = chunk_sum<rtg_bf16, KIND>(reinterpret_cast<const rtg_bf16*>(t.p[c.i]) + c.lo, c.n);
+  else acc = chunk_sum<float, KIND>(reinterpret_cast<const float*>(t.p[c.i]) + c.lo, c.n);
+  acc = block_join<KIND, THREADS>(acc, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+template <int KIND>
+__global__ __launch_bounds__(REDUCE) void grad_norm_finish(const double* __restrict__ part, int n, float* __restrict__ out) {
+  __shared__ double red[REDUCE / 64];
+  const double norm = norm_of<KIND>(all_partials<KIND, REDUCE>(part, n, red));
+  if (threadIdx.x == 0) *out = (float)norm;
+}
+
+template <class T>
+__device__ __forceinline__ void chunk_scale(T* __restrict__ p, long long n, float f) {
+  constexpr int N = RtgVec<T>::N;
+  const long long nv = n / N;
+  for (long long i = threadIdx.x; i < nv; i += THREADS) {
+    RtgVec<T> v;
+    float r[N];
+    v.load(p + i * N);
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = v.get(e) * f;
+    v.set(r);
+    v.store(p + i * N);
+  }
+  if (nv * N + threadIdx.x < n) rtg_down(rtg_up(p[nv * N + threadIdx.x]) * f, p[nv * N + threadIdx.x]);
+}
+
+// every workgroup joins the partials by itself (they sit in L2; a launch of one workgroup for it costs more) and scales the
+// chunk whose sum it may have taken
+template <int KIND>
+__global__ __launch_bounds__(THREADS) void grad_scale(const GradTable t, const double* __restrict__ part, int n_part, double max_norm,
+                                                      float* __restrict__ out, int write_norm) {
+  __shared__ double red[THREADS / 64];
+  const double norm = norm_of<KIND>(all_partials<KIND, THREADS>(part, n_part, red));
+  if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *out = (float)norm;
+  const float f = clip_factor(norm, max_norm);
+  if (f == 1.f) return;
+  const Piece c = piece_of(t);
+  if (c.bf) chunk_scale(reinterpret_cast<rtg_bf16*>(t.p[c.i]) + c.lo, c.n, f);
+  else chunk_scale(reinterpret_cast<float*>(t.p[c.i]) + c.lo, c.n, f);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// AdamW over flat buffers with clipped gradients: torch.optim.AdamW's order of operations (adamw_kernel, rtg_elem.hip)
+// ---------------------------------------------------------------------------------------------------------------------
+struct AdamTable {
+  RtgAdamWJob job[JOBS];
+  int first[JOBS];
+  int count;
+  long long chunk;                    // elements, a multiple of 1024
+};
+struct AdamScalars { float step_size, bc2s, scale, go; };        // go 0: the buffer is left alone
+
+// one workgroup between the norm and the update: the factor and each buffer's bias corrections once, in double; the step
+// counters advance here, behind the last reader of the old ones
+__global__ __launch_bounds__(REDUCE) void adam_prepare(const AdamTable t, const double* __restrict__ part, int n_part, double max_norm,
+                                                       double lr, double b1, double b2, float gscale, AdamScalars* __restrict__ sc,
+                                                       float* __restrict__ norm_out, int write_norm) {
+  __shared__ double red[REDUCE / 64];
+  const double norm = sqrt(all_partials<RTG_NORM_L2, REDUCE>(part, n_part, red)) * fabs((double)gscale);
+  const int j = threadIdx.x;
+  if (j == 0 && write_norm && norm_out) *norm_out = (float)norm;
+  if (j >= t.count) return;
+  const float* flag = t.job[j].loss_flag;
+  const bool go = isfinite(norm) && !(flag && isnan(*flag));
+  const double step = (double)t.job[j].step_state[0] + 1.0;
+  AdamScalars s;
+  s.step_size = (float)(lr / (1.0 - pow(b1, step)));
+  s.bc2s = (float)sqrt(1.0 - pow(b2, step));
+  s.scale = gscale * clip_factor(norm, max_norm);
+  s.go = go ? 1.f : 0.f;
+  sc[j] = s;
+  if (go) t.job[j].step_state[0] = (float)step;
+}
+
+__global__ __launch_bounds__(THREADS) void adam_update(const AdamTable t, const AdamScalars* __restrict__ sc, float w1, float b2, float w2,
+                                                       float decay, float eps) {
+  const int j = entry_of(t.first, t.count, blockIdx.x);
+  const AdamScalars s = sc[j];
+  if (s.go == 0.f) return;
+  const long long lo = (long long)((int)blockIdx.x - t.first[j]) * t.chunk;
+  const long long left = t.job[j].n - lo, n = left < t.chunk ? left : t.chunk;
+  float* const __restrict__ p = t.job[j].params + lo;
+  const float* const __restrict__ g = t.job[j].grads + lo;
+  float* const __restrict__ m = t.job[j].exp_avg + lo;
+  float* const __restrict__ v = t.job[j].exp_avg_sq + lo;
+  const auto step = [&](float& pi, float gi, float& mi, float& vi) __attribute__((always_inline)) {
+    gi *= s.scale;
+    mi = mi + w1 * (gi - mi);
+    vi = vi * b2 + w2 * gi * gi;
+    pi = pi * decay - s.step_size * mi / (sqrtf(vi) / s.bc2s + eps);
+  };
+  const long long nv = n / 4;
+  for (long long i = threadIdx.x; i < nv; i += THREADS) {
+    RtgVec<float> a, b, c, d;
+    a.load(p + 4 * i);
+    b.load(g + 4 * i);
+    c.load(m + 4 * i);
+    d.load(v + 4 * i);
+    float pr[4], mr[4], vr[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      pr[e] = a.get(e);
+      mr[e] = c.get(e);
+      vr[e] = d.get(e);
+      step(pr[e], b.get(e), mr[e], vr[e]);
+    }
+    a.set(pr);
+    c.set(mr);
+    d.set(vr);
+    a.store(p + 4 * i);
+    c.store(m + 4 * i);
+    d.store(v + 4 * i);
+  }
+  const long long i = 4 * nv + threadIdx.x;
+  if (i < n) step(p[i], g[i], m[i], v[i]);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int MAX_TENSORS = 1 << 20;
+
+// bytes of a chunk: about BLOCKS chunks over a long list, at least 16 KB (four rounds of a workgroup's loads)
+long long chunk_bytes(long long total) {
+  const long long c = (total / BLOCKS + 4095) / 4096 * 4096;
+  return c < 16384 ? 16384 : c;
+}
+
+// walks the list, TABLE tensors a launch: launch(table, workgroups, workgroups before) for each -> status; *blocks: all of them
+template <class F>
+int each_table(int n, void* const* grads, const long long* counts, const int* bf16, int* blocks, F launch) {
+  long long total = 0;
+  for (int i = 0; i < n; ++i) total += counts[i] * (bf16[i] ? 2 : 4);
+  GradTable t;
+  t.chunk = chunk_bytes(total);
+  int before = 0, here = 0;
+  t.count = 0;
+  for (int k = 0; k < TABLE / 32; ++k) t.bf16[k] = 0;
+  for (int i = 0; i <= n; ++i) {
+    if (t.count == TABLE || (i == n && t.count > 0)) {
+      const int rc = launch(t, here, before);
+      if (rc != RTG_OK) return rc;
+      before += here;
+      here = t.count = 0;
+      for (int k = 0; k < TABLE / 32; ++k) t.bf16[k] = 0;
+    }
+    if (i == n || counts[i] == 0) continue;
+    const long long bytes = counts[i] * (bf16[i] ? 2 : 4);
+    t.p[t.count] = grads[i];
+    t.n[t.count] = counts[i];
+    t.first[t.count] = here;
+    if (bf16[i]) t.bf16[t.count >> 5] |= 1u << (t.count & 31);
+    here += (int)((bytes + t.chunk - 1) / t.chunk);
+    ++t.count;
+  }
+  *blocks = before;
+  return RTG_OK;
+}
+
+int check_list(int n, void* const* grads, const long long* counts, const int* bf16, int kind, const void* ws) {
+  if (!grads || !counts || !bf16 || !ws) return RTG_ENULL;
+  if (n < 1 || n > MAX_TENSORS || (kind != RTG_NORM_L2 && kind != RTG_NORM_MAX)) return RTG_EINVAL;
+  long long total = 0;
+  for (int i = 0; i < n; ++i) {
+    if (counts[i] < 0) return RTG_EINVAL;
+    if (counts[i] > (1ll << 56) || (total += counts[i]) > (1ll << 56)) return RTG_ERANGE;
+    if (counts[i] > 0 && !grads[i]) return RTG_ENULL;
+    if (reinterpret_cast<uintptr_t>(grads[i]) & (bf16[i] ? 1 : 3)) return RTG_EINVAL;
+  }
+  return RTG_OK;
+}
+
+struct Range { uintptr_t lo, hi; };
+// no two ranges share a byte: workgroups of one launch would write what others read.  A list in the order of its addresses
+// (the views of a flat buffer) needs no sorting.
+int disjoint(Range* r, long long n) {
+  const auto ordered = [&]() {
+    for (long long i = 1; i < n; ++i)
+      if (r[i - 1].hi > r[i].lo) return false;
+    return true;
+  };
+  if (ordered()) return RTG_OK;
+  std::sort(r, r + n, [](const Range& a, const Range& b) { return a.lo < b.lo; });
+  return ordered() ? RTG_OK : RTG_EINVAL;
+}
+
+template <int KIND>
+int partials(int n, void* const* grads, const long long* counts, const int* bf16, double* ws, int* blocks, hipStream_t st) {
+  return each_table(n, grads, counts, bf16, blocks, [&](const GradTable& t, int here, int before) {
+    RTG_KLAUNCH(grad_partial<KIND>, dim3(here), dim3(THREADS), 0, st, t, ws + before);
+    return rtg_launch_status();
+  });
+}
+
+template <int KIND>
+int norm(int n, void* const* grads, const long long* counts, const int* bf16, double* ws, float* out, hipStream_t st) {
+  int blocks = 0;
+  const int rc = partials<KIND>(n, grads, counts, bf16, ws, &blocks, st);
+  if (rc != RTG_OK) return rc;
+  RTG_KLAUNCH(grad_norm_finish<KIND>, dim3(1), dim3(REDUCE), 0, st, (const double*)ws, blocks, out);
+  return rtg_launch_status();
+}
+
+template <int KIND>
+int clip(int n, void* const* grads, const long long* counts, const int* bf16, double max_norm, double* ws, float* out, hipStream_t st) {
+  int blocks = 0, again = 0;
+  const int rc = partials<KIND>(n, grads, counts, bf16, ws, &blocks, st);
+  if (rc != RTG_OK) return rc;
+  if (blocks == 0) {                                     // nothing but empty tensors: the norm is 0
+    RTG_KLAUNCH(grad_norm_finish<KIND>, dim3(1), dim3(REDUCE), 0, st, (const double*)ws, 0, out);
+    return rtg_launch_status();
+  }
+  return each_table(n, grads, counts, bf16, &again, [&](const GradTable& t, int here, int before) {
+    RTG_KLAUNCH(grad_scale<KIND>, dim3(here), dim3(THREADS), 0, st, t, (const double*)ws, blocks, max_norm, out, (int)(before == 0));
+    return rtg_launch_status();
+  });
+}
+
+}  // namespace
+
+extern "C" long long rtg_grad_ws(int n) {
+  if (n < 1 || n > MAX_TENSORS) return RTG_EINVAL;
+  // a partial per chunk (at most BLOCKS full ones and a last one per tensor), and AdamW's scalars
+  return (long long)BLOCKS + n + (long long)n * (sizeof(AdamScalars) / sizeof(double));
+}
+
+extern "C" int rtg_grad_norm(int n, const void* const* grads, const long long* counts, const int* bf16, int kind, double* ws,
+                             float* norm_out, void* stream) {
+  void* const* g = const_cast<void* const*>(grads);
+  const int rc = check_list(n, g, counts, bf16, kind, ws);
+  if (rc != RTG_OK) return rc;
+  if (!norm_out) return RTG_ENULL;
+  return kind == RTG_NORM_L2 ? norm<RTG_NORM_L2>(n, g, counts, bf16, ws, norm_out, (hipStream_t)stream)
+                             : norm<RTG_NORM_MAX>(n, g, counts, bf16, ws, norm_out, (hipStream_t)stream);
+}
+
+extern "C" int rtg_grad_clip(int n, void* const* grads, const long long* counts, const int* bf16, int kind, double max_norm, double* ws,
+                             float* norm_out, void* stream) {
+  const int rc = check_list(n, grads, counts, bf16, kind, ws);
+  if (rc != RTG_OK) return rc;
+  if (!norm_out) return RTG_ENULL;
+  if (!(max_norm >= 0.0)) return RTG_EINVAL;
+  {
+    std::unique_ptr<Range[]> r(new (std::nothrow) Range[n]);
+    if (!r) return RTG_ERANGE;
+    int k = 0;
+    for (int i = 0; i < n; ++i) {
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(grads[i]);
+      if (counts[i] > 0) r[k++] = Range{lo, lo + (uintptr_t)counts[i] * (bf16[i] ? 2 : 4)};
+    }
+    const int apart = disjoint(r.get(), k);
+    if (apart != RTG_OK) return apart;
+  }
+  return kind == RTG_NORM_L2 ? clip<RTG_NORM_L2>(n, grads, counts, bf16, max_norm, ws, norm_out, (hipStream_t)stream)
+                             : clip<RTG_NORM_MAX>(n, grads, counts, bf16, max_norm, ws, norm_out, (hipStream_t)stream);
+}
+
+extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm, double lr, double beta1, double beta2, double eps,
+                                 double weight_decay, float grad_scale, double* ws, float* norm_out, void* stream) {
+  if (!jobs || !ws) return RTG_ENULL;
+  if (n < 1 || n > MAX_TENSORS || !(max_norm >= 0.0)) return RTG_EINVAL;
+  long long total = 0;
+  for (int i = 0; i < n; ++i) {
+    const RtgAdamWJob& j = jobs[i];
+    if (!j.params || !j.grads || !j.exp_avg || !j.exp_avg_sq || !j.step_state) return RTG_ENULL;
+    if (j.n < 1) return RTG_EINVAL;
+    if (j.n > (1ll << 56) || (total += j.n) > (1ll << 56)) return RTG_ERANGE;
+    if ((reinterpret_cast<uintptr_t>(j.params) | reinterpret_cast<uintptr_t>(j.grads) | reinterpret_cast<uintptr_t>(j.exp_avg) |
+         reinterpret_cast<uintptr_t>(j.exp_avg_sq) | reinterpret_cast<uintptr_t>(j.step_state)) & 3) return RTG_EINVAL;
+  }
+  {
+    std::unique_ptr<Range[]> r(new (std::nothrow) Range[5 * (size_t)n]);
+    if (!r) return RTG_ERANGE;
+    for (int i = 0; i < n; ++i) {
+      const RtgAdamWJob& j = jobs[i];
+      const void* p[5] = {j.params, j.grads, j.exp_avg, j.exp_avg_sq, j.step_state};
+      for (int k = 0; k < 5; ++k) {
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(p[k]);
+        r[5 * (size_t)i + k] = Range{lo, lo + (k < 4 ? 4 * (uintptr_t)j.n : 4)};
+      }
+    }
+    const int apart = disjoint(r.get(), 5ll * n);
+    if (apart != RTG_OK) return apart;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  // the partials, TABLE buffers a launch
+  GradTable t;
+  t.chunk = chunk_bytes(4 * total);
+  for (int k = 0; k < TABLE / 32; ++k) t.bf16[k] = 0;
+  int blocks = 0;
+  for (int i = 0; i < n; i += TABLE) {
+    int here = 0;
+    for (t.count = 0; t.count < TABLE && i + t.count < n; ++t.count) {
+      const RtgAdamWJob& j = jobs[i + t.count];
+      t.p[t.count] = const_cast<float*>(j.grads);
+      t.n[t.count] = j.n;
+      t.first[t.count] = here;
+      here += (int)((4 * j.n + t.chunk - 1) / t.chunk);
+    }
+    RTG_KLAUNCH(grad_partial<RTG_NORM_L2>, dim3(here), dim3(THREADS), 0, st, t, ws + blocks);
+    const int rc = rtg_launch_status();
+    if (rc != RTG_OK) return rc;
+    blocks += here;
+  }
+  AdamScalars* sc = reinterpret_cast<AdamScalars*>(ws + BLOCKS + n);
+  AdamTable a;
+  a.chunk = t.chunk / 4;
+  for (int i = 0; i < n; i += JOBS) {
+    int here = 0;
+    for (a.count = 0; a.count < JOBS && i + a.count < n; ++a.count) {
+      a.job[a.count] = jobs[i + a.count];
+      a.first[a.count] = here;
+      here += (int)((jobs[i + a.count].n + a.chunk - 1) / a.chunk);
+    }
+    RTG_KLAUNCH(adam_prepare, dim3(1), dim3(REDUCE), 0, st, a, (const double*)ws, blocks, max_norm, lr, beta1, beta2, grad_scale, sc + i,
+                norm_out, (int)(i == 0));
+    int rc = rtg_launch_status();
+    if (rc != RTG_OK) return rc;
+    RTG_KLAUNCH(adam_update, dim3(here), dim3(THREADS), 0, st, a, (const AdamScalars*)(sc + i), (float)(1.0 - beta1), (float)beta2,
+                (float)(1.0 - beta2), (float)(1.0 - lr * weight_decay), (float)eps);
+    rc = rtg_launch_status();
+    if (rc != RTG_OK) return rc;
+  }
+  return RTG_OK;
+}

@@ -102,3 +102,7 @@ bf16_maps = False
 # resume schedule: False = the installed torch's ExponentialLR (2.x: the constructor leaves the loaded lr untouched);
 # True = torch 1.8's (the reference's README.md:15): one more factor of lr_decay per resume.  See train.ExponentialLR.
 legacy_resume_lr = False
+# largest 2-norm of an optimizer's gradients (all models of the optimizer together, the mean over the ranks): larger ones are
+# scaled down to it inside the update, and an update whose norm is not finite is left out (train.AdamW max_norm).  None: no
+# limit, the reference's behaviour.  Read when a Trainer is built.
+grad_clip = None

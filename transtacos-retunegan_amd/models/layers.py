@@ -58,6 +58,26 @@ class WNConv(nn.Module):
                 f'g={self.groups}')
 
 
+class LayerNorm(nn.Module):
+    """Layer norm over one axis (rtg.ops.layer_norm): dim=1, the channels of feature maps [B, C, T] or [B, C, H, W], or dim=-1,
+    the rows of [..., C].  Parameters named and initialised like torch.nn.LayerNorm's; inside a BankedModel they live in the
+    model's flat buffers (one optimizer launch, one all-reduce, one gradient norm with the convolutions' weights)."""
+
+    def __init__(self, channels, eps=1e-5, dim=1, affine=True, bias=True):
+        super().__init__()
+        self.channels, self.eps, self.dim = int(channels), float(eps), int(dim)
+        self.weight = nn.Parameter(torch.ones(self.channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(self.channels)) if affine and bias else None
+
+    def forward(self, x):
+        if x.dim() < 1 or not -x.dim() <= self.dim < x.dim() or x.shape[self.dim] != self.channels:
+            raise RtgError(f'LayerNorm({self.channels}, dim={self.dim}): got a tensor of shape {tuple(x.shape)}')
+        return ops.layer_norm(x, self.weight, self.bias, self.eps, self.dim)
+
+    def extra_repr(self):
+        return f'{self.channels}, eps={self.eps}, dim={self.dim}'
+
+
 class BankedModel(nn.Module):
     """nn.Module whose WNConv children (and listed extra parameters) live in one WeightBank on the GPU."""
 
@@ -69,7 +89,9 @@ class BankedModel(nn.Module):
         BankedModel._registry.add(self)
 
     def _extra_bank_params(self):
-        return []
+        """[(name, parameter)] besides the convolutions': those of the model's LayerNorm children (a model with more of them
+        appends its own to this list)"""
+        return [(f'{n}.{k}', p) for n, m in self.named_modules() if isinstance(m, LayerNorm) for k, p in m.named_parameters()]
 
     def _apply(self, fn, *a, **k):
         r = super()._apply(fn, *a, **k)

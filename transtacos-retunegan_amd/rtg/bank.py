@@ -463,6 +463,10 @@ class WeightBank:
     def flag(self):
         return self.gflat[self.n_params:]
 
+    def grads(self):
+        """the gradient buffer without the flag slot"""
+        return self.gflat[:self.n_params]
+
     def set_flag(self, loss):
         """store the (device scalar) loss of the step being differentiated in the flag slot"""
         src = loss.detach().reshape(1)

@@ -104,6 +104,16 @@ class StftBwdJob(C.Structure):      # RtgStftBwdJob (ABI 11)
                                                                'binmel_w', 'frame_ws')]
 
 
+class LayerNormDesc(C.Structure):
+    _fields_ = [(n, C.c_longlong) for n in ('outer', 'n', 'inner', 'x_outer', 'x_n')] + \
+               [('bf16', C.c_int), ('param_bf16', C.c_int), ('eps', C.c_float)]
+
+
+class AdamWJob(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ('params', 'grads', 'exp_avg', 'exp_avg_sq', 'step_state', 'loss_flag')] + \
+               [('n', C.c_longlong)]
+
+
 PRE_NONE, PRE_LRELU, PRE_MUL_DLRELU, PRE_MUL_DTANH = 0, 1, 2, 3
 ACT_NONE, ACT_LRELU, ACT_TANH = 0, 1, 2
 PACK_FWD, PACK_DGRAD_S1, PACK_DGRAD_POLY, PACK_CONVT_POLY, PACK_DGRAD_2D, PACK_GCONV_FWD, PACK_GCONV_BWD, PACK_GMFMA_FWD = 0, 1, 2, 3, 4, 5, 6, 7
@@ -111,6 +121,7 @@ IO_X_BF16, IO_OUT_BF16, IO_MASK_BF16, IO_RES_BF16 = 1, 2, 4, 8
 CK = 16
 LOSS_L1, LOSS_L1_L1LOG, LOSS_MSE_TARGET, LOSS_MSE_REL, LOSS_L1_ENC = 0, 1, 2, 3, 4
 MAX_LOSS_JOBS = 48
+NORM_L2, NORM_MAX = 0, 1
 
 ABI_VERSION = 11           # RTG_ABI_VERSION of include/rtg.h these struct layouts / prototypes were written for
 _P = C.c_void_p
@@ -171,6 +182,13 @@ PROTOTYPES = {
     'rtg_strip_mirror_fwd': (_I, [_P, _I, _I, _F, _P, _P, _P, _P]),
     'rtg_strip_mirror_bwd': (_I, [_P, _I, _I, _F, _P, _P, _P, _P]),
     'rtg_adamw': (_I, [_P, _P, _P, _P, _LL, _P, _P, _D, _D, _D, _D, _D, _F, _P]),
+    'rtg_layernorm_forward': (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P]),
+    'rtg_layernorm_ws': (_LL, [C.POINTER(LayerNormDesc)]),
+    'rtg_layernorm_backward': (_I, [C.POINTER(LayerNormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    'rtg_grad_ws': (_LL, [_I]),
+    'rtg_grad_norm': (_I, [_I, _P, _P, _P, _I, _P, _P, _P]),
+    'rtg_grad_clip': (_I, [_I, _P, _P, _P, _I, _D, _P, _P, _P]),
+    'rtg_adamw_clipped': (_I, [_I, _P, _D, _D, _D, _D, _D, _D, _F, _P, _P, _P]),
     'rtg_resstack_ok': (_I, [C.POINTER(ResStackDesc)]),
     'rtg_resstack_forward': (_I, [C.POINTER(ResStackDesc), _P, C.POINTER(PtrArray6), C.POINTER(PtrArray6), C.POINTER(PtrArray6), _P]),
     'rtg_resstack_backward': (_I, [C.POINTER(ResStackDesc), _P, _P, C.POINTER(PtrArray6), C.POINTER(PtrArray6), C.POINTER(PtrArray6), _P]),

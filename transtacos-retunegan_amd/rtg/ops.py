@@ -1302,6 +1302,275 @@ class PeriodFoldFn(torch.autograd.Function):
 
 
 # ---------------------------------------------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------------------------------------------
+_NORM_TYPES = (torch.float32, _BF)
+
+
+def _need_here(what, *ts):
+    """the kernels run on the current stream of the CURRENT device: every tensor has to live there"""
+    here = None
+    for t in ts:
+        if t is None:
+            continue
+        _need_cuda(t)
+        if here is None:
+            here = torch.cuda.current_device()
+        if t.get_device() != here:
+            raise L.RtgError(f'{what}: a tensor lives on {t.device}, the current device is cuda:{here} '
+                             '(call torch.cuda.set_device first: one process per GPU)')
+
+
+def _axes(shape, stride, lo, hi):
+    """dimensions [lo, hi) of a tensor as ONE axis -> (length, stride), or None where they do not collapse"""
+    n, st = 1, 1
+    for d in range(hi - 1, lo - 1, -1):
+        if shape[d] == 1:
+            continue
+        if n == 1:
+            st = stride[d]
+        elif stride[d] != st * n:
+            return None
+        n *= shape[d]
+    return n, st
+
+
+def _norm_desc(x, weight, eps, dim):
+    """(x as the kernels can read it, its descriptor): [outer][n][inner] around axis `dim`, copied only where the axes around it
+    do not collapse or the positions of a map are not adjacent"""
+    shape, bf, pbf = x.shape, int(_is_bf(x)), int(weight is not None and _is_bf(weight))
+    if x.numel() == 0:
+        return x, L.LayerNormDesc(0, shape[dim], 1, 0, 1, bf, pbf, eps)
+    for _ in range(2):                                     # (the second round: a contiguous copy)
+        stride = x.stride()
+        outer, inner = _axes(shape, stride, 0, dim), _axes(shape, stride, dim + 1, x.dim())
+        n = shape[dim]
+        if outer and inner and (inner[0] == 1 and (n == 1 or stride[dim] == 1) or inner[0] > 1 and inner[1] == 1):
+            break
+        x = x.contiguous()
+    return x, L.LayerNormDesc(outer[0], n, inner[0], outer[1], stride[dim] if n > 1 else 1, bf, pbf, eps)
+
+
+def _like_map(x):
+    return empty_bf(x.shape, x.device) if _is_bf(x) else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
+def _check_norm(x, weight, bias, eps, dim):
+    _need_here('layer_norm', x, weight, bias)
+    if x.dtype not in _NORM_TYPES:
+        raise L.RtgError(f'layer_norm: {x.dtype} activations (float32 or bfloat16)')
+    if x.dim() < 1 or not -x.dim() <= dim < x.dim():
+        raise L.RtgError(f'layer_norm: axis {dim} of a tensor of shape {tuple(x.shape)}')
+    n = x.shape[dim]
+    if n < 1:
+        raise L.RtgError(f'layer_norm: the normalised axis of {tuple(x.shape)} is empty')
+    if not 0.0 <= eps < float('inf'):
+        raise L.RtgError(f'layer_norm: eps {eps!r}')
+    for name, p in (('weight', weight), ('bias', bias)):
+        if p is not None and (tuple(p.shape) != (n,) or p.dtype not in _NORM_TYPES):
+            raise L.RtgError(f'layer_norm: {name} is {p.dtype} {tuple(p.shape)}, expected float32 or bfloat16 ({n},)')
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise L.RtgError(f'layer_norm: weight is {weight.dtype}, bias {bias.dtype}: expected one type')
+    return dim % x.dim()
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, dim=-1, keep=False):
+    """layer_norm without autograd -> y, or with `keep` (y, mean, rstd): the statistics (float32, one per row or position)
+    that layer_norm_backward reads"""
+    dim = _check_norm(x, weight, bias, eps, dim)
+    weight, bias = _c(weight), _c(bias)
+    x, d = _norm_desc(x, weight if weight is not None else bias, eps, dim)
+    y = _like_map(x)
+    mean = rstd = None
+    if keep:
+        mean, rstd = torch.empty(2, d.outer * d.inner, device=x.device).unbind(0)
+    size = 2 if d.bf16 else 4
+    check(timed_bw('layernorm_fwd', 2 * size * x.numel(), lambda: lib.rtg_layernorm_forward(
+        C.byref(d), _p(x), _p(weight), _p(bias), _p(y), _p(mean), _p(rstd), _stream())), 'layernorm forward')
+    return (y, mean, rstd) if keep else y
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, dim=-1, needs=(True, True, True), param_dtype=None):
+    """(dx, dweight, dbias) of layer_norm_forward(x, weight, bias, eps, dim, keep=True); `needs` says which are wanted (None in
+    the place of the others).  The gradients of weight and bias have weight's type (param_dtype where there is no weight)."""
+    dim = _check_norm(x, weight, None, 0.0, dim)
+    _need_here('layer_norm', dy, mean, rstd)
+    x, d = _norm_desc(x, weight, 0.0, dim)
+    rows = d.outer * d.inner
+    if dy.dtype != x.dtype or dy.shape != x.shape:
+        raise L.RtgError(f'layer_norm backward: dy is {dy.dtype} {tuple(dy.shape)}, the activations {x.dtype} {tuple(x.shape)}')
+    if not all(s.dtype == torch.float32 and s.numel() == rows and s.is_contiguous() for s in (mean, rstd)):
+        raise L.RtgError(f'layer_norm backward: mean and rstd have to be contiguous float32 tensors of {rows} elements')
+    weight, dy = _c(weight), _c(dy)
+    kind = weight.dtype if weight is not None else (param_dtype or torch.float32)
+    if kind not in _NORM_TYPES:
+        raise L.RtgError(f'layer_norm backward: gradients of type {kind} (float32 or bfloat16)')
+    d.param_bf16 = int(kind == _BF)
+    dx = _like_map(x) if needs[0] else None
+    dw = torch.empty(d.n, device=x.device, dtype=kind) if needs[1] else None
+    db = torch.empty(d.n, device=x.device, dtype=kind) if needs[2] else None
+    ws = None
+    if dw is not None or db is not None:
+        ws = torch.empty(lib.rtg_layernorm_ws(C.byref(d)), device=x.device)
+    size = 2 if d.bf16 else 4
+    check(timed_bw('layernorm_bwd', 3 * size * x.numel(), lambda: lib.rtg_layernorm_backward(
+        C.byref(d), _p(dy), _p(x), _p(mean), _p(rstd), _p(weight), _p(dx), _p(dw), _p(db), _p(ws), _stream())), 'layernorm backward')
+    return dx, dw, db
+
+
+class LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, dim):
+        y, mean, rstd = layer_norm_forward(x, weight, bias, eps, dim, keep=True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.cfg = (dim, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dim, kind = ctx.cfg
+        return (*layer_norm_backward(dy, x, mean, rstd, weight, dim, ctx.needs_input_grad[:3], kind), None, None)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
+    """(x - mean) / sqrt(var + eps) * weight + bias over axis `dim` (torch.nn.functional.layer_norm over one axis, any one of
+    them): dim=-1 for rows of activations, dim=1 for the channels of feature maps [B, C, T] / [B, C, H, W].  x: float32 or
+    bfloat16, taken as the values it holds (a bf16 map of the discriminators goes through ops.decode first); weight / bias:
+    float32 or bfloat16 of shape (n,), or None.  Strided rows, time crops and channel slices of a map are read in place, and a
+    map whose channels are adjacent ([B, T, C] transposed) takes the row kernels; the result is as dense as x is.  One launch
+    forward, two backward (gradients of x, weight and bias, summed in a fixed order); not differentiable twice."""
+    ts = (x, weight, bias)
+    d = _check_norm(x, weight, bias, eps, dim)
+    if d != x.dim() - 1 and x.stride(d) == 1 and x.shape[d] > 1:          # the channels are adjacent: rows
+        return layer_norm(x.movedim(d, -1), weight, bias, eps, -1).movedim(-1, d)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        return LayerNormFn.apply(x, weight, bias, eps, d)
+    return layer_norm_forward(x, weight, bias, eps, d)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the norm over many gradients, clipping by it, and the update that reads clipped gradients
+# ---------------------------------------------------------------------------------------------------------------
+def _dense(t):
+    """every element of t's storage range belongs to it once, in whatever order"""
+    n = 1
+    for st, size in sorted((st, size) for st, size in zip(t.stride(), t.shape) if size != 1):
+        if st != n:
+            return False
+        n *= size
+    return True
+
+
+def _norm_kind(norm_type):
+    if norm_type in (2, 2.0):
+        return L.NORM_L2
+    if norm_type in (float('inf'), 'inf'):
+        return L.NORM_MAX
+    raise L.RtgError(f'norm_type {norm_type!r}: 2 or inf')
+
+
+def _limit(max_norm):
+    if isinstance(max_norm, torch.Tensor) or not float(max_norm) >= 0.0:
+        raise L.RtgError(f'max_norm {max_norm!r}: a number that is not negative')
+    return float(max_norm)
+
+
+class _GradList:
+    """a list of gradients as the C entry points take it: three host arrays (`keep`: tensors that have to outlive the call)"""
+
+    def __init__(self, what, tensors, in_place):
+        ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+        if not ts:
+            raise L.RtgError(f'{what}: no gradients')
+        for i, t in enumerate(ts):
+            if t.dtype not in _NORM_TYPES or t.layout is not torch.strided:
+                raise L.RtgError(f'{what}: gradient {i} is {t.dtype}, {t.layout} (float32 or bfloat16, strided)')
+            if not t.is_contiguous() and not _dense(t):
+                if in_place:
+                    raise L.RtgError(f'{what}: gradient {i} of shape {tuple(t.shape)} and strides {t.stride()} has gaps or overlaps '
+                                     'itself: it cannot be scaled in place')
+                ts[i] = t.contiguous()
+        _need_here(what, *ts)
+        n = len(ts)
+        self.n, self.keep, self.device = n, ts, ts[0].device
+        self.ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in ts])
+        self.counts = (C.c_longlong * n)(*[t.numel() for t in ts])
+        self.bf16 = (C.c_int * n)(*[t.dtype is _BF for t in ts])
+        self.bytes = sum(t.numel() * t.element_size() for t in ts) if PROFILE is not None else 0
+
+    def ws(self):
+        return torch.empty(lib.rtg_grad_ws(self.n), device=self.device, dtype=torch.float64)
+
+
+def total_norm(tensors, norm_type=2.0):
+    """The norm of all elements of a list of gradients together (torch.nn.utils.get_total_norm): norm_type 2 (squares and sums
+    in 64 bits: no gradient that a float holds overflows) or inf.  float32 and bfloat16 tensors, mixed as they come -> a float32
+    device scalar.  Nothing synchronises with the host."""
+    kind = _norm_kind(norm_type)
+    g = _GradList('total_norm', tensors, False)
+    ws, out = g.ws(), torch.empty((), device=g.device)
+    check(timed_bw('grad_norm', g.bytes, lambda: lib.rtg_grad_norm(g.n, g.ptrs, g.counts, g.bf16, kind, _p(ws), _p(out), _stream())),
+          'grad_norm')
+    return out
+
+
+def clip_grads_(grads, max_norm, norm_type=2.0):
+    """Scale a list of gradients in place by min(1, max_norm / (norm + 1e-6)) -> their norm before (a float32 device scalar):
+    what torch.nn.utils.clip_grad_norm_ does to the .grad of its parameters (train.clip_grad_norm_ takes parameters), on the
+    device alone.  A norm within the limit costs one read of the gradients and no write.  An infinite norm scales by 0, a
+    NaN by NaN, as torch's does."""
+    kind, limit = _norm_kind(norm_type), _limit(max_norm)
+    g = _GradList('clip_grads_', grads, True)
+    ws, out = g.ws(), torch.empty((), device=g.device)
+    check(timed_bw('grad_clip', 2 * g.bytes, lambda: lib.rtg_grad_clip(g.n, g.ptrs, g.counts, g.bf16, kind, limit, _p(ws), _p(out),
+                                                                       _stream())), 'grad_clip (do gradients overlap?)')
+    torch.autograd.graph.increment_version(g.keep)
+    return out
+
+
+def clipped_adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, max_norm, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                   grad_scale=1.0, loss_flags=None, out=None):
+    """One AdamW update (train.AdamW: torch.optim.AdamW's arithmetic) of a list of flat float32 buffers with their gradients
+    clipped to max_norm over ALL of them -> the norm of grads * grad_scale before (`out`, or a new device scalar).  The factor
+    is applied where the update reads the gradients: they keep their values and are not written.  steps: one float32 device
+    scalar per buffer, advanced by the call; loss_flags: None, or per buffer a device scalar (or None) whose NaN leaves that
+    buffer, its moments and its step alone.  A norm that is not finite leaves all of them alone."""
+    limit = _limit(max_norm)
+    cols = [list(c) for c in (params, grads, exp_avgs, exp_avg_sqs, steps)]
+    n = len(cols[0])
+    flags = [None] * n if loss_flags is None else list(loss_flags)
+    if n < 1 or any(len(c) != n for c in cols) or len(flags) != n:
+        raise L.RtgError(f'clipped_adamw_: lists of {[len(c) for c in cols]} buffers and {len(flags)} loss flags')
+    if not grad_scale > 0.0:
+        raise L.RtgError(f'clipped_adamw_: grad_scale {grad_scale!r}')
+    jobs = (L.AdamWJob * n)()
+    for i, (p, g, m, v, t) in enumerate(zip(*cols)):
+        _need_here('clipped_adamw_', p, g, m, v, t, flags[i])
+        if any(b.dtype != torch.float32 or not b.is_contiguous() or b.numel() != p.numel() for b in (p, g, m, v)) or p.numel() < 1:
+            raise L.RtgError(f'clipped_adamw_: buffer {i}: parameters, gradients and moments have to be contiguous float32 tensors '
+                             'of one size')
+        if any(b is not None and (b.dtype != torch.float32 or b.numel() != 1) for b in (t, flags[i])):
+            raise L.RtgError(f'clipped_adamw_: buffer {i}: the step and the loss flag have to be float32 scalars on the device')
+        jobs[i] = L.AdamWJob(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), t.data_ptr(),
+                             None if flags[i] is None else flags[i].data_ptr(), p.numel())
+    dev = cols[0][0].device
+    if out is None:
+        out = torch.empty((), device=dev)
+    else:
+        _need_here('clipped_adamw_', out)
+        if out.dtype != torch.float32 or out.numel() != 1:
+            raise L.RtgError('clipped_adamw_: out has to be a float32 scalar on the device')
+    ws = torch.empty(lib.rtg_grad_ws(n), device=dev, dtype=torch.float64)
+    check(timed_bw('adamw_clipped', 32 * sum(p.numel() for p in cols[0]), lambda: lib.rtg_adamw_clipped(
+        n, jobs, limit, lr, betas[0], betas[1], eps, weight_decay, grad_scale, _p(ws), _p(out), _stream())),
+          'adamw_clipped (do buffers overlap?)')
+    torch.autograd.graph.increment_version(cols[0] + cols[2] + cols[3] + cols[4])
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------
 # losses (multi-tensor)
 # ---------------------------------------------------------------------------------------------------------------
 def _jobs(entries):

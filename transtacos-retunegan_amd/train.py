@@ -74,7 +74,11 @@ class AdamW:
     buffers of one or more BankedModels: ONE kernel launch per model instead of 550 per-tensor updates per step
     (SURVEY.md 2.1).  Constructible like the reference does it: AdamW(module.parameters(), lr, betas=[b1, b2])."""
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None):
+        """max_norm: bound of the 2-norm of grad * grad_scale over ALL the optimizer's models; larger gradients are scaled to it
+        where the update reads them (rtg.ops.clipped_adamw_), an update with a norm that is not finite is left out.  After a
+        step `total_norm` holds the norm before (a device scalar, one buffer for all steps).  Like lr, max_norm is a launch
+        argument: a captured step keeps the value it was captured with."""
         params = list(params)
         if params and isinstance(params[0], BankedModel):
             models = params
@@ -94,6 +98,8 @@ class AdamW:
         self.param_groups = [{'lr': self.lr, 'betas': self.betas, 'eps': eps, 'weight_decay': weight_decay,
                               'initial_lr': self.lr}]
         self.grad_scale = 1.0
+        self.max_norm = None if max_norm is None else ops._limit(max_norm)
+        self.total_norm = None
 
     def _st(self, m):
         bank = m.bank()
@@ -118,15 +124,28 @@ class AdamW:
         use_bank_flag: test the flag slot of each model's gradient buffer instead (WeightBank.set_flag: the loss value
         rides the data-parallel all-reduce of the gradients, so the guard is collective without a collective of its own)."""
         lr = self.param_groups[0]['lr']
+        if self.max_norm is not None and self.models:
+            return self._step_clipped(lr, loss_flag, use_bank_flag)
         for m in self.models:
             s = self._st(m)
             bank = s['bank']
             bank.sync_grads()
-            from rtg import ops
             check(ops.timed_bw('adamw', 28 * bank.n_params, lambda: lib.rtg_adamw(
                 _p(bank.flat), _p(bank.gflat), _p(s['exp_avg']), _p(s['exp_avg_sq']), bank.n_params, _p(s['step']),
                 _p(bank.flag() if use_bank_flag else loss_flag), lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, self.grad_scale,
                 _stream()), type(m).__name__), 'adamw')
+
+    def _step_clipped(self, lr, loss_flag, use_bank_flag):
+        st = [self._st(m) for m in self.models]
+        banks = [s['bank'] for s in st]
+        for b in banks:
+            b.sync_grads()
+        if self.total_norm is None or self.total_norm.device != banks[0].device:
+            self.total_norm = torch.zeros((), device=banks[0].device)
+        flags = [b.flag() for b in banks] if use_bank_flag else [loss_flag] * len(banks)
+        ops.clipped_adamw_([b.flat for b in banks], [b.grads() for b in banks], [s['exp_avg'] for s in st],
+                           [s['exp_avg_sq'] for s in st], [s['step'] for s in st], self.max_norm, lr=lr, betas=self.betas, eps=self.eps,
+                           weight_decay=self.weight_decay, grad_scale=self.grad_scale, loss_flags=flags, out=self.total_norm)
 
     def step_tensor(self, m=None):
         return self._st(m or self.models[0])['step']
@@ -171,6 +190,25 @@ class AdamW:
         self.param_groups[0]['lr'] = float(g['lr'])
         if 'initial_lr' in g:
             self.initial_lr = self.param_groups[0]['initial_lr'] = float(g['initial_lr'])
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
+    """torch.nn.utils.clip_grad_norm_ on the device: the .grad of `parameters` (an iterable of parameters, one of them, or whole
+    BankedModels) scaled in place to a norm of at most max_norm -> their norm before, a device scalar (rtg.ops.clip_grads_).
+    Gradients still on their way from a backward pass are waited for on the device.  Parameters without a gradient are passed
+    over; none left: 0."""
+    items = [parameters] if isinstance(parameters, (torch.Tensor, BankedModel)) else list(parameters)
+    params = {}                                                # each parameter once, in the order given
+    for p in items:
+        for q in (p.parameters() if isinstance(p, BankedModel) else (p,)):
+            params[id(q)] = q
+    for m in list(BankedModel._registry):
+        if m._bank is not None and any(id(p) in params for p in m._bank.params):
+            m._bank.sync_grads()                               # the last flush may sit on a forked stream
+    grads = [p.grad for p in params.values() if p.grad is not None]
+    if not grads:
+        return torch.zeros((), device=next(iter(params.values())).device if params else device)
+    return ops.clip_grads_(grads, max_norm, norm_type)
 
 
 class ExponentialLR:
@@ -315,9 +353,10 @@ class Trainer:
         self.mtd = (mtd or MultiStftDiscriminator()).to(dev) if use_mtd else None
         self.discs = [d for d in (self.msd, self.mpd, self.mtd) if d is not None]
         self.d_train_times = hp.d_train_times if d_train_times is None else d_train_times
-        self.optim_g = AdamW(self.generator.parameters(), hp.learning_rate_g, betas=[hp.adam_b1, hp.adam_b2])
+        clip = getattr(hp, 'grad_clip', None)
+        self.optim_g = AdamW(self.generator.parameters(), hp.learning_rate_g, betas=[hp.adam_b1, hp.adam_b2], max_norm=clip)
         self.optim_d = AdamW(itertools.chain(*[d.parameters() for d in self.discs]), hp.learning_rate_d,
-                             betas=[hp.adam_b1, hp.adam_b2])
+                             betas=[hp.adam_b1, hp.adam_b2], max_norm=clip)
         self.scheduler_g = ExponentialLR(self.optim_g, gamma=hp.lr_decay)
         self.scheduler_d = ExponentialLR(self.optim_d, gamma=hp.lr_decay)
         self.dp = DataParallel([self.generator, *self.discs], process_group)
