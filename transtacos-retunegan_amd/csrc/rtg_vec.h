@@ -17,7 +17,12 @@ __device__ __forceinline__ void rtg_down(float v, float& out) { out = v; }
 // (bf16: round to nearest even, the one rounding of a result)
 __device__ __forceinline__ void rtg_down(float v, rtg_bf16& out) { out.u = __builtin_bit_cast(unsigned short, (__bf16)v); }
 
-// VEC elements of T as they lie in memory
+// the value is computed here, not later (volatile statements keep their order)
+__device__ __forceinline__ void rtg_pin(float& v) { asm volatile("" : "+v"(v)); }
+
+// N elements of T as they lie in memory.  hold(): the compiler forgets what it has computed from the vector, so a kernel that
+// reads its tile several times converts it again (a shift an element) instead of keeping every element's float in a register;
+// behind rtg_pin of what was summed from it (else the sums move behind hold() and the vector is kept twice).
 template <class T> struct RtgVec;
 template <> struct RtgVec<float> {
   static constexpr int N = 4;
@@ -30,7 +35,7 @@ template <> struct RtgVec<float> {
     for (int e = 0; e < 4; ++e) r[e] = __float_as_uint(v[e]);
   }
   __device__ __forceinline__ void zero() { r = u32x4{0, 0, 0, 0}; }
-  __device__ __forceinline__ void put(int e, float v) { r[e] = __float_as_uint(v); }
+  __device__ __forceinline__ void hold() {}
 };
 template <> struct RtgVec<rtg_bf16> {
   static constexpr int N = 8;
@@ -49,4 +54,5 @@ template <> struct RtgVec<rtg_bf16> {
     }
   }
   __device__ __forceinline__ void zero() { r = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void hold() { asm volatile("" : "+v"(r)); }
 };
