@@ -31,6 +31,12 @@ __device__ __forceinline__ float param_at(const void* p, int bf, long long i, fl
   return bf ? rtg_up(reinterpret_cast<const rtg_bf16*>(p)[i]) : reinterpret_cast<const float*>(p)[i];
 }
 
+__device__ __forceinline__ void put_param(void* p, int bf, long long i, float v) {
+  if (!p) return;
+  if (bf) rtg_down(v, reinterpret_cast<rtg_bf16*>(p)[i]);
+  else reinterpret_cast<float*>(p)[i] = v;
+}
+
 // N parameters from index i on as floats (all of them exist); `dflt` where there are none
 template <int N>
 __device__ __forceinline__ void load_params(float (&out)[N], const void* p, int bf, long long i, float dflt) {
@@ -52,13 +58,23 @@ __device__ __forceinline__ void load_params(float (&out)[N], const void* p, int 
   }
 }
 
+template <int N>
+__device__ __forceinline__ void store_floats(const float (&v)[N], float* p) {
+#pragma unroll
+  for (int k = 0; k < N / 4; ++k) {
+    RtgVec<float> r;
+    r.set({v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]});
+    r.store(p + 4 * k);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // The register kernels.  All their accesses are whole vectors: where an axis ends inside a lane's vector, the lane's vector ends
 // with the axis instead and repeats `dup` elements of the lane before it.  Those elements come out the same from both (each is
 // computed from sums that everyone has in one order), so writing them twice is harmless; only sums leave the repeated ones out.
 // A lane that lies behind the axis as a whole (dup >= N) loads what the last one loads and adds and writes nothing.
 //
-// Rows.  TPR threads hold a row in registers, VPT 16-byte vectors each, so x is read once; the sums are shuffles inside a wave
+// Rows.  TPR threads hold a row in registers, VPT 16-byte vectors each, so x is read once; the sums are lane swaps inside a wave
 // and, for rows longer than a wave holds, one round through LDS each.  A block walks rows with the weights in registers and
 // the next row's loads in flight while it works on this one.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -73,9 +89,7 @@ __device__ __forceinline__ void pin_all(float (&v)[K]) {
 template <int TPR, int BLK, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[BLK / 64]) {
 #pragma unroll
-  for (int off = (TPR < 64 ? TPR : 64) / 2; off > 0; off >>= 1)
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], off, 64);
+  for (int k = 0; k < K; ++k) v[k] = rtg_group_sum<(TPR < 64 ? TPR : 64)>(v[k]);
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     const int wave = threadIdx.x >> 6, first = wave / W * W;
@@ -189,7 +203,7 @@ __global__ __launch_bounds__(BLK) void ln_row_fwd(LnShape s, const T* __restrict
 template <class T, int TPR, int VPT, int BLK, int AHEAD>
 __global__ __launch_bounds__(BLK) void ln_row_bwd(LnShape s, const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean_in,
                                                   const float* __restrict__ rstd_in, const void* __restrict__ w, T* __restrict__ dx,
-                                                  float* __restrict__ part) {
+                                                  float* __restrict__ part, void* __restrict__ dw, void* __restrict__ db) {
   constexpr int N = RtgVec<T>::N, G = BLK / TPR, E = VPT * N;
   __shared__ float red[2][2][BLK / 64];
   __shared__ float sums[G > 1 ? E * BLK : 1];
@@ -267,26 +281,38 @@ __global__ __launch_bounds__(BLK) void ln_row_bwd(LnShape s, const T* __restrict
   if (!part) return;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    float* out = part + ((long long)blockIdx.x * 2 + which) * s.n;
-    if constexpr (G == 1) {
-#pragma unroll
-      for (int k = 0; k < VPT; ++k)
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (e >= at.dup[k]) out[at.col[k] + e] = which ? ab[k][e] : aw[k][e];
-    } else {
+    float* const out = part + ((long long)blockIdx.x * 2 + which) * s.n;
+    if constexpr (G > 1) {
+      // (the column order of the vectors, so that both sides of the exchange go through LDS in adjacent words)
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
 #pragma unroll
-        for (int e = 0; e < N; ++e) sums[(k * N + e) * BLK + threadIdx.x] = which ? ab[k][e] : aw[k][e];
+        for (int e = 0; e < N; ++e) sums[g * (TPR * E) + (k * TPR + t) * N + e] = which ? ab[k][e] : aw[k][e];
       __syncthreads();
-      for (int j = threadIdx.x; j < E * TPR; j += BLK) {
-        const int k = j / (N * TPR), e = j / TPR % N, tt = j % TPR, nominal = (k * TPR + tt) * N, n = (int)s.n;
-        const int col = nominal < n - N ? nominal : n - N;
+      for (int j = threadIdx.x; j < TPR * E; j += BLK) {
+        const int at0 = j / N * N, n = (int)s.n, col = at0 < n - N ? at0 : n - N;
         float a = 0.f;
-        for (int i = 0; i < G; ++i) a += sums[(k * N + e) * BLK + i * TPR + tt];
-        if (e >= nominal - col) out[col + e] = a;
+#pragma unroll
+        for (int i = 0; i < G; ++i) a += sums[i * (TPR * E) + j];
+        if (j % N < at0 - col) continue;
+        if (gridDim.x > 1) out[col + j % N] = a;
+        else put_param(which ? db : dw, s.pbf, col + j % N, a);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        float(&v)[N] = which ? ab[k] : aw[k];
+        if (gridDim.x > 1 && at.dup[k] == 0) {
+          store_floats<N>(v, out + at.col[k]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (e >= at.dup[k]) {
+              if (gridDim.x > 1) out[at.col[k] + e] = v[e];
+              else put_param(which ? db : dw, s.pbf, at.col[k] + e, v[e]);
+            }
+        }
       }
     }
   }
@@ -297,24 +323,25 @@ __global__ __launch_bounds__(BLK) void ln_row_bwd(LnShape s, const T* __restrict
 // CPT channels each in registers; W waves share the channels of a tile where one cannot hold them.  Every load is a whole
 // 16 * LP bytes of a channel's row, CPT of them in flight per lane.
 // ---------------------------------------------------------------------------------------------------------------------
-// sums of K values per position over the channel lanes of a wave and the W waves of a team
+// workgroup b of a grid of 8 k runs on XCD b % 8 (each has its own L2): neighbours in the order of the tiles are put on one XCD, so
+// a line that two tiles share — rows of a map that do not start on a line — is fetched once
+__device__ __forceinline__ unsigned xcd_order(unsigned b, unsigned grid) { return b % 8 * (grid / 8) + b / 8; }
+
+// K sums over the channel lanes of a wave and the W waves of a team, scattered over the lanes (rtg_scatter_sum)
 template <int LP, int W, int K>
-__device__ __forceinline__ void tile_sum(float (&v)[K], float (*red)[K * LP + 1]) {
-#pragma unroll
-  for (int off = LP; off < 64; off <<= 1)
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], off, 64);
+__device__ __forceinline__ void tile_sum(float (&v)[K], float (*red)[64 * rtg_scattered(LP, K)]) {
+  constexpr int R = rtg_scattered(LP, K);
+  rtg_scatter_sum<LP, K>(v);
   if constexpr (W > 1) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = wave / W * W;
-    if (lane < LP)
 #pragma unroll
-      for (int k = 0; k < K; ++k) red[wave][k * LP + lane] = v[k];
+    for (int k = 0; k < R; ++k) red[wave][k * 64 + lane] = v[k];
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+    for (int k = 0; k < R; ++k) {
       v[k] = 0.f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) v[k] += red[first + i][k * LP + lane % LP];
+      for (int i = 0; i < W; ++i) v[k] += red[first + i][k * 64 + lane];
     }
   }
 }
@@ -326,16 +353,6 @@ struct MapTile {
   static constexpr int N = RtgVec<T>::N, CL = 64 / LP, TEAMS = map_teams(W), BLK = map_block(W);
   static constexpr int POS = LP * N, CH = CL * W * CPT;
 };
-
-template <int N>
-__device__ __forceinline__ void store_floats(const float (&v)[N], float* p) {
-#pragma unroll
-  for (int k = 0; k < N / 4; ++k) {
-    RtgVec<float> r;
-    r.set({v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]});
-    r.store(p + 4 * k);
-  }
-}
 
 // where a lane of a tile stands.  The wave's part of every address is scalar, a lane's is 32 bits; a lane without a channel
 // works on channel lane 0's (of the last channel, where the wave has none) for nothing
@@ -415,10 +432,11 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_fwd(LnShape s, const T* _
                                                                            float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   using M = MapTile<T, LP, W, CPT>;
   constexpr int N = M::N;
-  __shared__ float red[2][W > 1 ? M::BLK / 64 : 1][N * LP + 1];
+  constexpr int R = rtg_scattered(LP, N);
+  __shared__ float red[2][W > 1 ? M::BLK / 64 : 1][64 * R];
   MapLane<T, LP, W, CPT> at(s);
   const unsigned per = (unsigned)((s.inner + M::POS - 1) / M::POS);
-  at.go(s, blockIdx.x * M::TEAMS + at.wave / W, (unsigned)s.outer * per, per);
+  at.go(s, xcd_order(blockIdx.x, gridDim.x) * M::TEAMS + at.wave / W, (unsigned)s.outer * per, per);
   RtgVec<T> v[CPT];
   at.load(v, x, s.xo, s.xn);
   float wr[CPT], br[CPT], a[N], mean[N], rstd[N];
@@ -435,10 +453,10 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_fwd(LnShape s, const T* _
   }
   tile_sum<LP, W, N>(a, red[0]);
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    mean[e] = mean_of(a[e], s);
-    a[e] = 0.f;
-  }
+  for (int k = 0; k < R; ++k) mean[k] = mean_of(a[k], s);
+  rtg_gather<LP, N>(mean);
+#pragma unroll
+  for (int e = 0; e < N; ++e) a[e] = 0.f;
 #pragma unroll
   for (int i = 0; i < CPT; ++i) {
 #pragma unroll
@@ -451,7 +469,8 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_fwd(LnShape s, const T* _
   }
   tile_sum<LP, W, N>(a, red[1]);
 #pragma unroll
-  for (int e = 0; e < N; ++e) rstd[e] = rstd_of(a[e], s);
+  for (int k = 0; k < R; ++k) rstd[k] = rstd_of(a[k], s);
+  rtg_gather<LP, N>(rstd);
   at.store(y, s.n * s.inner, s.inner, [&](int i) __attribute__((always_inline)) {
     float r[N];
 #pragma unroll
@@ -474,7 +493,8 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* _
                                                                            float* __restrict__ part) {
   using M = MapTile<T, LP, W, CPT>;
   constexpr int N = M::N;
-  __shared__ float red[2][W > 1 ? M::BLK / 64 : 1][2 * N * LP + 1];
+  constexpr int R = rtg_scattered(LP, 2 * N);
+  __shared__ float red[2][W > 1 ? M::BLK / 64 : 1][64 * R];
   __shared__ float sums[2][M::TEAMS][M::CH];
   MapLane<T, LP, W, CPT> at(s);
   const int team = at.wave / W;
@@ -484,7 +504,7 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* _
 #pragma unroll
   for (int i = 0; i < CPT; ++i) aw[i] = ab[i] = 0.f;
   int turn = 0;
-  for (unsigned base = blockIdx.x * M::TEAMS; base < tiles; base += gridDim.x * M::TEAMS, turn ^= 1) {
+  for (unsigned base = xcd_order(blockIdx.x, gridDim.x) * M::TEAMS; base < tiles; base += gridDim.x * M::TEAMS, turn ^= 1) {
     at.go(s, base + team, tiles, per);
     RtgVec<T> xv[CPT], gv[CPT];
     at.load(xv, x, s.xo, s.xn);
@@ -513,7 +533,8 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* _
     if (!dx) continue;
     tile_sum<LP, W, 2 * N>(a, red[turn]);
 #pragma unroll
-    for (int e = 0; e < 2 * N; ++e) a[e] *= s.inv_n;
+    for (int k = 0; k < R; ++k) a[k] *= s.inv_n;
+    rtg_gather<LP, 2 * N>(a);
     at.store(dx, s.n * s.inner, s.inner, [&](int i) __attribute__((always_inline)) {
       float r[N];
 #pragma unroll
@@ -723,12 +744,22 @@ __global__ __launch_bounds__(FIN_COLS* FIN_ROWS) void ln_finish(const float* __r
                                                                 void* __restrict__ dw, void* __restrict__ db, int pbf) {
   __shared__ float red[FIN_ROWS][FIN_COLS + 1];
   void* const out = blockIdx.y ? db : dw;
-  if (!out) return;
+  if (!out) return;                                        // (the whole block)
   const int col = threadIdx.x % FIN_COLS, r = threadIdx.x / FIN_COLS;
   const long long i = (long long)blockIdx.x * FIN_COLS + col;
   float acc = 0.f;
-  if (i < n)
-    for (int q = r; q < slices; q += FIN_ROWS) acc += part[((long long)q * 2 + blockIdx.y) * n + i];
+  if (i < n) {
+    const float* p = part + (long long)blockIdx.y * n + i;
+    int q = r;
+    for (; q + 7 * FIN_ROWS < slices; q += 8 * FIN_ROWS) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = p[(long long)(q + k * FIN_ROWS) * 2 * n];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc += v[k];
+    }
+    for (; q < slices; q += FIN_ROWS) acc += p[(long long)q * 2 * n];
+  }
   red[r][col] = acc;
   __syncthreads();
 #pragma unroll
@@ -736,10 +767,7 @@ __global__ __launch_bounds__(FIN_COLS* FIN_ROWS) void ln_finish(const float* __r
     if (r < h) red[r][col] += red[r + h][col];
     __syncthreads();
   }
-  if (r == 0 && i < n) {
-    if (pbf) rtg_down(red[0][col], reinterpret_cast<rtg_bf16*>(out)[i]);
-    else reinterpret_cast<float*>(out)[i] = red[0][col];
-  }
+  if (r == 0 && i < n) put_param(out, pbf, i, red[0][col]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -769,43 +797,86 @@ bool is_rows(const RtgLayerNormDesc* d) { return d->inner == 1; }
 struct Plan { int tile; int blocks; };
 constexpr int LOOPS = -1;
 
-// rows: threads per row and 16-byte vectors per thread.  Rows of up to 64 vectors leave no lane of a group idle for the sake of
-// a shuffle tree; past four vectors a thread (the weights' registers) a row goes to a whole block.
-struct RowTile { int tpr, vpt; };
-constexpr RowTile FWD_TILES[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}};
-// backward: sixteen elements a thread (weight, dw and db are three registers each)
-constexpr RowTile BWD_F32[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {512, 4}, {1024, 3}};
-constexpr RowTile BWD_BF16[] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}, {1024, 2}};
+// Rows: threads per row, 16-byte vectors per thread, threads per block.  Over 13 widths from 64 to 16384 and row counts from 1 to
+// 65536 these tiles are within 5 % of the best of 20 (forward) and 40 (backward); what they weigh: a wave's rows need no
+// barrier (up to two vectors a thread), a block's row two; the backward holds sixteen elements a thread at most (the weight, dw
+// and db take a register each); half the blocks that fit are enough where each walks its rows with the next in flight
+// (65536 x 1024 floats 91 us, with all of them 99).
+struct RowTile { int tpr, vpt, blk; };
+constexpr int ROW_TILES = 10;
+constexpr RowTile FWD_TILES[ROW_TILES] = {{8, 1, 256},   {16, 1, 256},  {32, 1, 256},  {64, 1, 256},   {64, 2, 256},
+                                          {256, 1, 256}, {256, 2, 256}, {512, 2, 512}, {1024, 2, 1024}, {1024, 4, 1024}};
+constexpr RowTile BWD_F32[ROW_TILES] = {{8, 1, 512},    {16, 1, 512},  {32, 1, 512},  {64, 1, 512},    {64, 2, 512},
+                                        {256, 1, 1024}, {256, 2, 512}, {512, 2, 512}, {1024, 2, 1024}, {1024, 3, 1024}};
+constexpr RowTile BWD_BF16[ROW_TILES] = {{8, 1, 512},   {16, 1, 512},  {32, 1, 512},  {64, 1, 512},    {64, 2, 512},
+                                         {256, 1, 512}, {256, 2, 512}, {512, 2, 512}, {1024, 2, 1024}, {1024, 2, 1024}};
 
 int row_tile(const RowTile* tiles, long long n, int bf16) {
   const int vec = bf16 ? 8 : 4;
   if (n < vec) return LOOPS;
   const long long nv = (n + vec - 1) / vec;
-  for (int i = 0; i < 10; ++i)
+  for (int i = 0; i < ROW_TILES; ++i)
     if (nv <= tiles[i].tpr * tiles[i].vpt) return i;
   return LOOPS;
 }
 
-// maps: position lanes, waves that share the channels, channels a lane (backward: x and dy are both held, eight channels a lane)
-struct MapCfg { int lp, w, cpt; };
-constexpr MapCfg MAP_FWD[] = {{2, 1, 4}, {2, 1, 16}, {2, 2, 16}, {32, 1, 8}, {8, 1, 4}, {8, 1, 8}, {8, 1, 16}, {8, 2, 16}, {8, 4, 16}, {8, 8, 16}};
-constexpr MapCfg MAP_BWD[] = {{2, 1, 4}, {2, 1, 8}, {2, 2, 8}, {2, 4, 8}, {32, 1, 8}, {8, 1, 4}, {8, 1, 8}, {8, 2, 8}, {8, 4, 8}, {8, 8, 8}, {4, 8, 8}};
+// Maps: position lanes, waves that share the channels, channels a lane, as one number (the dispatch's label).  Over 12 channel
+// counts from 8 to 1024 and 7 sizes of map each, both types, the rules below are 2 % (forward) and 3 % (backward) behind the best
+// of all 38 tiles; what they weigh:
+//   - the channels are just covered: 32 channels by 8 x 4 lanes' worth 14.9 us of a 67 MB map, by twice as many 17.3;
+//   - a wide tile (a line of 128 bytes of each channel, 16 channels a lane: few waves meet for a sum) where its waves fill the
+//     chip twice: 128 channels x 65536 positions 13.5 us against 17.4 with four channels a lane and four waves; with 1024
+//     positions it is the other way round, 4.6 against 3.6: more waves, fewer loads each;
+//   - two position lanes where a clip has no more than two vectors of positions (512 channels x 8: 3.7 us against 4.2).
+constexpr int map_key(int lp, int w, int cpt) { return lp * 10000 + w * 100 + cpt; }
+#define LN_MAP_FWD(X) \
+  X(16, 1, 2) X(16, 1, 4) X(8, 1, 4) X(8, 2, 4) X(8, 4, 4) X(4, 4, 4) X(4, 8, 4) X(2, 1, 4) X(2, 2, 4) X(2, 4, 4) X(2, 8, 4) \
+  X(8, 1, 8) X(8, 1, 16) X(8, 2, 16) X(8, 4, 16) X(8, 8, 16)
+#define LN_MAP_BWD(X) \
+  X(16, 1, 2) X(16, 1, 4) X(8, 1, 4) X(8, 2, 4) X(8, 4, 4) X(8, 8, 4) X(4, 4, 4) X(4, 8, 4) X(2, 1, 4) X(2, 2, 4) X(2, 4, 4) X(2, 8, 4) \
+  X(8, 2, 8) X(8, 8, 8) X(4, 8, 8)
 
-struct MapPlan { int i; long long blocks; };               // blocks: enough for one tile a team
-template <int COUNT>
-MapPlan map_tile(const MapCfg (&cfg)[COUNT], const RtgLayerNormDesc* d) {
-  const int vec = d->bf16 ? 8 : 4;
-  if (d->inner < vec || d->inner >= 1 << 24 || d->x_n >= 1 << 24) return {LOOPS, 0};      // (a lane's offset in a tile has 32 bits)
-  for (int i = 0; i < COUNT; ++i) {
-    const MapCfg& m = cfg[i];
-    if (m.lp == 2 ? d->inner > 2 * vec : d->inner <= 2 * vec) continue;
-    if (m.lp == 32 && d->inner < 32 * vec) continue;       // few channels and many positions: more positions a wave
-    if (d->n > 64 / m.lp * m.w * m.cpt) continue;
-    const long long pos = m.lp * vec, tiles = d->outer * ((d->inner + pos - 1) / pos), teams = map_teams(m.w);
-    if (tiles >= 1ll << 30) return {LOOPS, 0};
-    return {i, (tiles + teams - 1) / teams};
-  }
-  return {LOOPS, 0};
+long long map_tiles(const RtgLayerNormDesc* d, int lp) {
+  const long long pos = lp * (d->bf16 ? 8 : 4);
+  return d->outer * ((d->inner + pos - 1) / pos);
+}
+// two of a wide tile's waves for every SIMD (256 CUs of four)
+bool map_wide(const RtgLayerNormDesc* d, int lp, int w) { return map_tiles(d, lp) * w >= 2048; }
+
+int map_fwd(const RtgLayerNormDesc* d) {
+  const long long n = d->n;
+  if (d->inner <= (d->bf16 ? 16 : 8))
+    return n <= 128 ? map_key(2, 1, 4) : n <= 256 ? map_key(2, 2, 4) : n <= 512 ? map_key(2, 4, 4) : map_key(2, 8, 4);
+  if (n <= 8) return map_key(16, 1, 2);
+  if (n <= 16) return map_key(16, 1, 4);
+  if (n <= 32) return map_key(8, 1, 4);
+  if (n <= 64) return map_wide(d, 8, 1) ? map_key(8, 1, 8) : map_key(8, 2, 4);
+  if (n <= 128) return map_wide(d, 8, 1) ? map_key(8, 1, 16) : map_key(8, 4, 4);
+  if (n <= 256) return map_wide(d, 8, 2) ? map_key(8, 2, 16) : map_key(4, 4, 4);
+  if (n <= 512) return map_wide(d, 8, 4) ? map_key(8, 4, 16) : map_tiles(d, 8) >= 64 ? map_key(4, 8, 4) : map_key(2, 4, 4);
+  return map_wide(d, 8, 8) ? map_key(8, 8, 16) : map_key(2, 8, 4);
+}
+
+int map_bwd(const RtgLayerNormDesc* d) {
+  const long long n = d->n;
+  if (d->inner <= (d->bf16 ? 16 : 8))
+    return n <= 128 ? map_key(2, 1, 4) : n <= 256 ? map_key(2, 2, 4) : n <= 512 ? map_key(2, 4, 4) : map_key(2, 8, 4);
+  if (n <= 8) return map_key(16, 1, 2);
+  if (n <= 16) return map_key(16, 1, 4);
+  if (n <= 32) return map_key(8, 1, 4);
+  if (n <= 64) return map_key(8, 2, 4);
+  if (n <= 128) return map_wide(d, 8, 1) ? map_key(8, 2, 8) : map_key(8, 4, 4);
+  if (n <= 256) return map_wide(d, 8, 8) ? map_key(8, 8, 4) : map_key(4, 4, 4);
+  if (n <= 512) return map_wide(d, 8, 2) ? map_key(8, 8, 8) : map_key(4, 8, 4);
+  return map_wide(d, 4, 8) ? map_key(4, 8, 8) : map_key(2, 8, 4);
+}
+
+// blocks that give each team one tile; 0: no register tile holds the problem (or a lane's offset in a tile would pass 32 bits)
+long long map_blocks(const RtgLayerNormDesc* d, int key) {
+  const int channels = 64 / (key / 10000) * (key / 100 % 100) * (key % 100);
+  if (d->inner < (d->bf16 ? 8 : 4) || d->n > channels || d->inner >= 1 << 24 || d->x_n >= 1 << 24) return 0;
+  const long long tiles = map_tiles(d, key / 10000), teams = map_teams(key / 100 % 100);
+  return tiles >= 1ll << 30 ? 0 : (tiles + teams - 1) / teams;
 }
 
 // blocks for `items` tiles of work, at most `cap` of them with as even a share as can be
@@ -814,19 +885,17 @@ int even_blocks(long long items, long long cap) {
   return (int)((items + rounds - 1) / rounds);
 }
 
-constexpr int row_block(int tpr) { return tpr <= 256 ? 256 : tpr; }
-constexpr int row_block_bwd(int tpr) { return tpr <= 512 ? 512 : tpr; }
-
 Plan plan_fwd(const RtgLayerNormDesc* d) {
   if (is_rows(d)) {
     const int i = row_tile(FWD_TILES, d->n, d->bf16);
     if (i == LOOPS) return {LOOPS, (int)lmin(d->outer, 1 << 20)};
-    const int blk = row_block(FWD_TILES[i].tpr), groups = blk / FWD_TILES[i].tpr;
-    return {i, even_blocks((d->outer + groups - 1) / groups, 256 * (2048 / blk))};
+    const int groups = FWD_TILES[i].blk / FWD_TILES[i].tpr;
+    return {i, even_blocks((d->outer + groups - 1) / groups, 256 * (1024 / FWD_TILES[i].blk))};
   }
-  const MapPlan m = map_tile(MAP_FWD, d);
-  if (m.i == LOOPS) return {LOOPS, (int)lmin(d->outer * ((d->inner + 63) / 64), 1 << 20)};
-  return {m.i, (int)m.blocks};
+  const int key = map_fwd(d);
+  const long long blocks = map_blocks(d, key);
+  if (blocks == 0) return {LOOPS, (int)lmin(d->outer * ((d->inner + 63) / 64), 1 << 20)};
+  return {key, ((int)blocks + 7) / 8 * 8};
 }
 
 Plan plan_bwd(const RtgLayerNormDesc* d) {
@@ -834,14 +903,18 @@ Plan plan_bwd(const RtgLayerNormDesc* d) {
     const RowTile* tiles = d->bf16 ? BWD_BF16 : BWD_F32;
     const int i = row_tile(tiles, d->n, d->bf16);
     if (i != LOOPS) {
-      const int blk = row_block_bwd(tiles[i].tpr), groups = blk / tiles[i].tpr;
-      return {i, even_blocks((d->outer + groups - 1) / groups, 512)};
+      // 256 blocks: two partials a CU would be more to add than the second block gains.  One block alone writes dw and db
+      // itself; it is worth that for a few rounds of rows (16 x 512: 4.4 us, in two blocks and ln_finish 5.7).
+      const int groups = tiles[i].blk / tiles[i].tpr;
+      const long long rounds = (d->outer + groups - 1) / groups;
+      return {i, rounds <= (tiles[i].tpr <= 64 ? 4 : 1) ? 1 : even_blocks(rounds, 256)};
     }
     const long long cols = (d->n + 63) / 64, s = lmin((d->outer + 15) / 16, (2048 + cols - 1) / cols);
     return {LOOPS, (int)(s < 1 ? 1 : lmin(s, 1024))};
   }
-  const MapPlan m = map_tile(MAP_BWD, d);
-  if (m.i != LOOPS) return {m.i, even_blocks(m.blocks, MAP_BWD[m.i].w > 4 ? 256 : 512)};
+  const int key = map_bwd(d);
+  const long long blocks = map_blocks(d, key);
+  if (blocks > 0) return {key, (even_blocks(blocks, key / 100 % 100 * (key % 100) >= 64 ? 256 : 512) + 7) / 8 * 8};
   const long long s = lmin((d->outer * d->inner + 1023) / 1024, (2048 + d->n - 1) / d->n);
   return {LOOPS, (int)(s < 1 ? 1 : lmin(s, 1024))};
 }
@@ -852,41 +925,25 @@ int forward(const RtgLayerNormDesc* d, const void* x, const void* w, const void*
   const T* xt = reinterpret_cast<const T*>(x);
   T* yt = reinterpret_cast<T*>(y);
   const Plan p = plan_fwd(d);
-#define LN_ROW(I, TPR, VPT)                                                                                                  \
-  case I:                                                                                                                    \
-    RTG_KLAUNCH((ln_row_fwd<T, TPR, VPT, row_block(TPR), (TPR * VPT < 4096)>), dim3(p.blocks), dim3(row_block(TPR)), 0, st, s, xt, \
-                w, b, yt, mean, rstd);                                                                                       \
-    return rtg_launch_status()
-#define LN_MAP(I, LP, W, CPT)                                                                                                \
-  case I:                                                                                                                    \
+#define LN_ROW(I)                                                                                                            \
+  case I: {                                                                                                                  \
+    constexpr RowTile R = FWD_TILES[I];                                                                                      \
+    RTG_KLAUNCH((ln_row_fwd<T, R.tpr, R.vpt, R.blk, (R.tpr * R.vpt < 4096)>), dim3(p.blocks), dim3(R.blk), 0, st, s, xt, w, b, yt, \
+                mean, rstd);                                                                                                 \
+    return rtg_launch_status();                                                                                              \
+  }
+#define LN_MAP(LP, W, CPT)                                                                                                   \
+  case map_key(LP, W, CPT):                                                                                                                    \
     RTG_KLAUNCH((ln_map_fwd<T, LP, W, CPT>), dim3(p.blocks), dim3(map_block(W)), 0, st, s, xt, w, b, yt, mean, rstd); \
-    return rtg_launch_status()
+    return rtg_launch_status();
   if (is_rows(d)) {
     switch (p.tile) {
-      LN_ROW(0, 8, 1);
-      LN_ROW(1, 16, 1);
-      LN_ROW(2, 32, 1);
-      LN_ROW(3, 64, 1);
-      LN_ROW(4, 64, 2);
-      LN_ROW(5, 64, 4);
-      LN_ROW(6, 256, 2);
-      LN_ROW(7, 256, 4);
-      LN_ROW(8, 1024, 2);
-      LN_ROW(9, 1024, 4);
+      LN_ROW(0) LN_ROW(1) LN_ROW(2) LN_ROW(3) LN_ROW(4) LN_ROW(5) LN_ROW(6) LN_ROW(7) LN_ROW(8) LN_ROW(9)
     }
     RTG_KLAUNCH(ln_row_loop_fwd<T>, dim3(p.blocks), dim3(LOOP_THREADS), 0, st, s, xt, w, b, yt, mean, rstd);
   } else {
     switch (p.tile) {
-      LN_MAP(0, 2, 1, 4);
-      LN_MAP(1, 2, 1, 16);
-      LN_MAP(2, 2, 2, 16);
-      LN_MAP(3, 32, 1, 8);
-      LN_MAP(4, 8, 1, 4);
-      LN_MAP(5, 8, 1, 8);
-      LN_MAP(6, 8, 1, 16);
-      LN_MAP(7, 8, 2, 16);
-      LN_MAP(8, 8, 4, 16);
-      LN_MAP(9, 8, 8, 16);
+      LN_MAP_FWD(LN_MAP)
     }
     RTG_KLAUNCH(ln_map_loop_fwd<T>, dim3(p.blocks), dim3(LOOP_THREADS), 0, st, s, xt, w, b, yt, mean, rstd);
   }
@@ -905,28 +962,20 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
   if (!dx && !params) return RTG_OK;
   float* const part = params ? ws : nullptr;
   const Plan p = plan_bwd(d);
-#define LN_ROW(I, TPR, VPT, AHEAD)                                                                                           \
-  case I:                                                                                                                    \
-    RTG_KLAUNCH((ln_row_bwd<T, TPR, VPT, row_block_bwd(TPR), AHEAD>), dim3(p.blocks), dim3(row_block_bwd(TPR)), 0, st, s, gt, \
-                xt, mean, rstd, w, dt, part);                                                                                \
-    break
-#define LN_MAP(I, LP, W, CPT)                                                                                                \
-  case I:                                                                                                                    \
+#define LN_ROW(I)                                                                                                            \
+  case I: {                                                                                                                  \
+    constexpr RowTile R = sizeof(T) == 2 ? BWD_BF16[I] : BWD_F32[I];                                                         \
+    RTG_KLAUNCH((ln_row_bwd<T, R.tpr, R.vpt, R.blk, (R.tpr < 1024)>), dim3(p.blocks), dim3(R.blk), 0, st, s, gt, xt, mean, rstd, w, \
+                dt, part, dw, db);                                                                                           \
+    break;                                                                                                                   \
+  }
+#define LN_MAP(LP, W, CPT)                                                                                                   \
+  case map_key(LP, W, CPT):                                                                                                                    \
     RTG_KLAUNCH((ln_map_bwd<T, LP, W, CPT>), dim3(p.blocks), dim3(map_block(W)), 0, st, s, gt, xt, mean, rstd, w, dt, part); \
-    break
-  constexpr bool BF = sizeof(T) == 2;
+    break;
   if (is_rows(d) && p.tile != LOOPS) {
     switch (p.tile) {
-      LN_ROW(0, 8, 1, 1);
-      LN_ROW(1, 16, 1, 1);
-      LN_ROW(2, 32, 1, 1);
-      LN_ROW(3, 64, 1, 1);
-      LN_ROW(4, 64, 2, 1);
-      LN_ROW(5, (BF ? 256 : 64), (BF ? 1 : 4), 1);
-      LN_ROW(6, 256, 2, 1);
-      LN_ROW(7, (BF ? 512 : 256), (BF ? 2 : 4), 1);
-      LN_ROW(8, (BF ? 1024 : 512), (BF ? 2 : 4), (BF ? 0 : 1));
-      LN_ROW(9, 1024, (BF ? 2 : 3), 0);
+      LN_ROW(0) LN_ROW(1) LN_ROW(2) LN_ROW(3) LN_ROW(4) LN_ROW(5) LN_ROW(6) LN_ROW(7) LN_ROW(8) LN_ROW(9)
     }
   } else if (is_rows(d)) {
     if (dx) {
@@ -938,17 +987,7 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
       RTG_KLAUNCH(ln_row_loop_dw<T>, dim3((unsigned)((d->n + 63) / 64), p.blocks), dim3(LOOP_THREADS), 0, st, s, gt, xt, mean, rstd, part, p.blocks);
   } else if (p.tile != LOOPS) {
     switch (p.tile) {
-      LN_MAP(0, 2, 1, 4);
-      LN_MAP(1, 2, 1, 8);
-      LN_MAP(2, 2, 2, 8);
-      LN_MAP(3, 2, 4, 8);
-      LN_MAP(4, 32, 1, 8);
-      LN_MAP(5, 8, 1, 4);
-      LN_MAP(6, 8, 1, 8);
-      LN_MAP(7, 8, 2, 8);
-      LN_MAP(8, 8, 4, 8);
-      LN_MAP(9, 8, 8, 8);
-      LN_MAP(10, 4, 8, 8);
+      LN_MAP_BWD(LN_MAP)
     }
   } else {
     if (dx) {
@@ -963,7 +1002,7 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
 #undef LN_ROW
 #undef LN_MAP
   const int rc = rtg_launch_status();
-  if (rc != RTG_OK || !params) return rc;
+  if (rc != RTG_OK || !params || (is_rows(d) && p.tile != LOOPS && p.blocks == 1)) return rc;   // (one block: dw, db are written)
   RTG_KLAUNCH(ln_finish, dim3((unsigned)rtg_ceil_div(d->n, FIN_COLS), 2), dim3(FIN_COLS * FIN_ROWS), 0, st, (const float*)ws, p.blocks,
               d->n, dw, db, s.pbf);
   return rtg_launch_status();
