@@ -45,7 +45,7 @@ def test_a_banked_model_lists_its_layer_norms():
 
 def test_axes_around_the_normalised_one():
     """what the kernels read in place, and what is copied first"""
-    from rtg.ops import _axes, _norm_desc
+    from rtg.ops import _axes, _norm_operands
     t = torch.zeros(6, 40, 90)
     assert _axes((6, 40), (3600, 90), 0, 2) == (240, 90) and _axes((6, 1, 40), (3600, 7, 90), 0, 3) == (240, 90)
     assert _axes((6, 40), (90, 540), 0, 2) is None and _axes((), (), 0, 0) == (1, 1)
@@ -55,7 +55,8 @@ def test_axes_around_the_normalised_one():
                                (t[:1, :1].expand(6, 40, 90), 2, (240, 90, 1, 0, 1), True),
                                (t[:, :, ::2], 1, (6, 40, 45, 1800, 45), False), (t.permute(1, 0, 2), 2, (240, 90, 1, 90, 1), False),
                                (t[:0], 2, (0, 90, 1, 0, 1), True)):
-        y, d = _norm_desc(x, None, 1e-5, dim)
+        y, p = _norm_operands(x, None, 1e-5, dim)
+        d = p.desc
         assert (d.outer, d.n, d.inner, d.x_outer, d.x_n) == want and (y.data_ptr() == x.data_ptr()) == same, (tuple(x.shape), dim)
 
 

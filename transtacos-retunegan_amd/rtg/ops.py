@@ -1,6 +1,9 @@
 """Autograd wrappers over the C ABI of librtg.so (include/rtg.h).  Every function here launches hand-written HIP
 kernels on the current torch stream; PyTorch only owns the memory and the autograd graph.  CPU tensors are refused."""
+import array
 import ctypes as C
+import functools
+import operator
 import os as _os
 
 import torch
@@ -1313,8 +1316,8 @@ def _need_here(what, *ts):
     for t in ts:
         if t is None:
             continue
-        _need_cuda(t)
         if here is None:
+            _need_cuda(*ts)
             here = torch.cuda.current_device()
         if t.get_device() != here:
             raise L.RtgError(f'{what}: a tensor lives on {t.device}, the current device is cuda:{here} '
@@ -1335,31 +1338,50 @@ def _axes(shape, stride, lo, hi):
     return n, st
 
 
-def _norm_desc(x, weight, eps, dim):
-    """(x as the kernels can read it, its descriptor): [outer][n][inner] around axis `dim`, copied only where the axes around it
-    do not collapse or the positions of a map are not adjacent"""
-    shape, bf, pbf = x.shape, int(_is_bf(x)), int(weight is not None and _is_bf(weight))
-    if x.numel() == 0:
-        return x, L.LayerNormDesc(0, shape[dim], 1, 0, 1, bf, pbf, eps)
-    for _ in range(2):                                     # (the second round: a contiguous copy)
-        stride = x.stride()
-        outer, inner = _axes(shape, stride, 0, dim), _axes(shape, stride, dim + 1, x.dim())
-        n = shape[dim]
-        if outer and inner and (inner[0] == 1 and (n == 1 or stride[dim] == 1) or inner[0] > 1 and inner[1] == 1):
-            break
+class _NormPlan:
+    """what a layer norm of one shape, layout and type needs besides its operands: [outer][n][inner] around the normalised axis
+    for the kernels, or desc None where they cannot read the activations in place (the axes around the normalised one do not
+    collapse, or the positions of a map are not adjacent)"""
+
+    def __init__(self, shape, stride, dim, bf, pbf, eps):
+        n, numel = shape[dim], 1
+        for size in shape:
+            numel *= size
+        outer, inner = _axes(shape, stride, 0, dim), _axes(shape, stride, dim + 1, len(shape))
+        self.desc, self.n, self.elements = None, n, numel
+        if numel == 0:
+            self.desc = L.LayerNormDesc(0, n, 1, 0, 1, bf, pbf, eps)
+        elif outer and inner and (inner[0] == 1 and (n == 1 or stride[dim] == 1) or inner[0] > 1 and inner[1] == 1):
+            self.desc = L.LayerNormDesc(outer[0], n, inner[0], outer[1], stride[dim] if n > 1 else 1, bf, pbf, eps)
+        if self.desc is not None:
+            self.rows = self.desc.outer * self.desc.inner
+            self.ref = C.byref(self.desc)
+            self.ws = None                                      # (floats of scratch of the backward, asked for when there is one)
+
+    def scratch(self):
+        if self.ws is None:
+            self.ws = lib.rtg_layernorm_ws(self.ref)
+        return self.ws
+
+
+_norm_plan = functools.lru_cache(maxsize=4096)(_NormPlan)
+
+
+def _norm_operands(x, kind, eps, dim):
+    """(x as the kernels can read it, the plan): copied only where they cannot; kind: the parameters' type"""
+    p = _norm_plan(x.shape, x.stride(), dim, x.dtype is _BF, kind is _BF, eps)
+    if p.desc is None:
         x = x.contiguous()
-    return x, L.LayerNormDesc(outer[0], n, inner[0], outer[1], stride[dim] if n > 1 else 1, bf, pbf, eps)
-
-
-def _like_map(x):
-    return empty_bf(x.shape, x.device) if _is_bf(x) else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        p = _norm_plan(x.shape, x.stride(), dim, x.dtype is _BF, kind is _BF, eps)
+    return x, p
 
 
 def _check_norm(x, weight, bias, eps, dim):
     _need_here('layer_norm', x, weight, bias)
     if x.dtype not in _NORM_TYPES:
         raise L.RtgError(f'layer_norm: {x.dtype} activations (float32 or bfloat16)')
-    if x.dim() < 1 or not -x.dim() <= dim < x.dim():
+    dims = x.dim()
+    if dims < 1 or not -dims <= dim < dims:
         raise L.RtgError(f'layer_norm: axis {dim} of a tensor of shape {tuple(x.shape)}')
     n = x.shape[dim]
     if n < 1:
@@ -1367,27 +1389,53 @@ def _check_norm(x, weight, bias, eps, dim):
     if not 0.0 <= eps < float('inf'):
         raise L.RtgError(f'layer_norm: eps {eps!r}')
     for name, p in (('weight', weight), ('bias', bias)):
-        if p is not None and (tuple(p.shape) != (n,) or p.dtype not in _NORM_TYPES):
+        if p is not None and (p.shape != (n,) or p.dtype not in _NORM_TYPES):
             raise L.RtgError(f'layer_norm: {name} is {p.dtype} {tuple(p.shape)}, expected float32 or bfloat16 ({n},)')
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise L.RtgError(f'layer_norm: weight is {weight.dtype}, bias {bias.dtype}: expected one type')
-    return dim % x.dim()
+    return dim % dims
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _norm_forward(x, weight, bias, eps, dim, keep):
+    """checked operands -> (y, statistics [mean | rstd] or None, x as read, the plan)"""
+    weight, bias = _c(weight), _c(bias)
+    like = weight if weight is not None else bias
+    x, p = _norm_operands(x, None if like is None else like.dtype, eps, dim)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    stats = torch.empty(2 * p.rows, device=x.device) if keep else None
+    mean = stats.data_ptr() if keep else None
+    rstd = mean + 4 * p.rows if keep else None
+    st = timed_bw('layernorm_fwd', 2 * x.element_size() * p.elements, lambda: lib.rtg_layernorm_forward(
+        p.ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean, rstd, _stream()))
+    if st:
+        check(st, 'layernorm forward')
+    return y, stats, x, p
+
+
+def _norm_backward(dy, x, mean, rstd, weight, p, kind, needs):
+    """mean, rstd: addresses; p: the plan of x with parameter gradients of type `kind`"""
+    dy, weight = _c(dy), _c(weight)
+    dev = x.device
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if needs[0] else None
+    dw = torch.empty(p.n, device=dev, dtype=kind) if needs[1] else None
+    db = torch.empty(p.n, device=dev, dtype=kind) if needs[2] else None
+    ws = torch.empty(p.scratch(), device=dev) if needs[1] or needs[2] else None
+    st = timed_bw('layernorm_bwd', 3 * x.element_size() * p.elements, lambda: lib.rtg_layernorm_backward(
+        p.ref, dy.data_ptr(), x.data_ptr(), mean, rstd, _ptr(weight), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), _stream()))
+    if st:
+        check(st, 'layernorm backward')
+    return dx, dw, db
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, dim=-1, keep=False):
     """layer_norm without autograd -> y, or with `keep` (y, mean, rstd): the statistics (float32, one per row or position)
     that layer_norm_backward reads"""
-    dim = _check_norm(x, weight, bias, eps, dim)
-    weight, bias = _c(weight), _c(bias)
-    x, d = _norm_desc(x, weight if weight is not None else bias, eps, dim)
-    y = _like_map(x)
-    mean = rstd = None
-    if keep:
-        mean, rstd = torch.empty(2, d.outer * d.inner, device=x.device).unbind(0)
-    size = 2 if d.bf16 else 4
-    check(timed_bw('layernorm_fwd', 2 * size * x.numel(), lambda: lib.rtg_layernorm_forward(
-        C.byref(d), _p(x), _p(weight), _p(bias), _p(y), _p(mean), _p(rstd), _stream())), 'layernorm forward')
-    return (y, mean, rstd) if keep else y
+    y, stats, _, p = _norm_forward(x, weight, bias, eps, _check_norm(x, weight, bias, eps, dim), keep)
+    return (y, stats[:p.rows], stats[p.rows:]) if keep else y
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, dim=-1, needs=(True, True, True), param_dtype=None):
@@ -1395,43 +1443,35 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, dim=-1, needs=(True, Tru
     the place of the others).  The gradients of weight and bias have weight's type (param_dtype where there is no weight)."""
     dim = _check_norm(x, weight, None, 0.0, dim)
     _need_here('layer_norm', dy, mean, rstd)
-    x, d = _norm_desc(x, weight, 0.0, dim)
-    rows = d.outer * d.inner
-    if dy.dtype != x.dtype or dy.shape != x.shape:
-        raise L.RtgError(f'layer_norm backward: dy is {dy.dtype} {tuple(dy.shape)}, the activations {x.dtype} {tuple(x.shape)}')
-    if not all(s.dtype == torch.float32 and s.numel() == rows and s.is_contiguous() for s in (mean, rstd)):
-        raise L.RtgError(f'layer_norm backward: mean and rstd have to be contiguous float32 tensors of {rows} elements')
-    weight, dy = _c(weight), _c(dy)
     kind = weight.dtype if weight is not None else (param_dtype or torch.float32)
     if kind not in _NORM_TYPES:
         raise L.RtgError(f'layer_norm backward: gradients of type {kind} (float32 or bfloat16)')
-    d.param_bf16 = int(kind == _BF)
-    dx = _like_map(x) if needs[0] else None
-    dw = torch.empty(d.n, device=x.device, dtype=kind) if needs[1] else None
-    db = torch.empty(d.n, device=x.device, dtype=kind) if needs[2] else None
-    ws = None
-    if dw is not None or db is not None:
-        ws = torch.empty(lib.rtg_layernorm_ws(C.byref(d)), device=x.device)
-    size = 2 if d.bf16 else 4
-    check(timed_bw('layernorm_bwd', 3 * size * x.numel(), lambda: lib.rtg_layernorm_backward(
-        C.byref(d), _p(dy), _p(x), _p(mean), _p(rstd), _p(weight), _p(dx), _p(dw), _p(db), _p(ws), _stream())), 'layernorm backward')
-    return dx, dw, db
+    if dy.dtype != x.dtype or dy.shape != x.shape:
+        raise L.RtgError(f'layer_norm backward: dy is {dy.dtype} {tuple(dy.shape)}, the activations {x.dtype} {tuple(x.shape)}')
+    x, p = _norm_operands(x, kind, 0.0, dim)
+    if not all(s.dtype == torch.float32 and s.numel() == p.rows and s.is_contiguous() for s in (mean, rstd)):
+        raise L.RtgError(f'layer_norm backward: mean and rstd have to be contiguous float32 tensors of {p.rows} elements')
+    return _norm_backward(dy, x, mean.data_ptr(), rstd.data_ptr(), weight, p, kind, needs)
 
 
 class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, dim):
-        y, mean, rstd = layer_norm_forward(x, weight, bias, eps, dim, keep=True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.cfg = (dim, None if bias is None else bias.dtype)
+        y, stats, x, ctx.plan = _norm_forward(x, weight, bias, eps, dim, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.kind = weight.dtype if weight is not None else (torch.float32 if bias is None else bias.dtype)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        dim, kind = ctx.cfg
-        return (*layer_norm_backward(dy, x, mean, rstd, weight, dim, ctx.needs_input_grad[:3], kind), None, None)
+        if torch.is_grad_enabled():                             # (create_graph: refuse to be differentiated once more)
+            return LayerNormFn.once(ctx, dy)
+        x, weight, stats = ctx.saved_tensors
+        p = ctx.plan
+        mean = stats.data_ptr()
+        return (*_norm_backward(dy, x, mean, mean + 4 * p.rows, weight, p, ctx.kind, ctx.needs_input_grad), None, None)
+
+    once = staticmethod(torch.autograd.function.once_differentiable(lambda ctx, dy: LayerNormFn.backward(ctx, dy)))
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
@@ -1441,13 +1481,13 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
     float32 or bfloat16 of shape (n,), or None.  Strided rows, time crops and channel slices of a map are read in place, and a
     map whose channels are adjacent ([B, T, C] transposed) takes the row kernels; the result is as dense as x is.  One launch
     forward, two backward (gradients of x, weight and bias, summed in a fixed order); not differentiable twice."""
-    ts = (x, weight, bias)
     d = _check_norm(x, weight, bias, eps, dim)
     if d != x.dim() - 1 and x.stride(d) == 1 and x.shape[d] > 1:          # the channels are adjacent: rows
         return layer_norm(x.movedim(d, -1), weight, bias, eps, -1).movedim(-1, d)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
         return LayerNormFn.apply(x, weight, bias, eps, d)
-    return layer_norm_forward(x, weight, bias, eps, d)
+    return _norm_forward(x, weight, bias, eps, d, False)[0]
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -1477,27 +1517,39 @@ def _limit(max_norm):
     return float(max_norm)
 
 
+_TB = torch._C.TensorBase
+_dtype_of, _layout_of = operator.attrgetter('dtype'), operator.attrgetter('layout')
+
+
 class _GradList:
-    """a list of gradients as the C entry points take it: three host arrays (`keep`: tensors that have to outlive the call)"""
+    """a list of gradients as the C entry points take it: three host arrays (`keep`: tensors that have to outlive the call).
+    A model has hundreds of them: whole-list passes of built-in methods, single tensors are looked at only to say what is wrong"""
 
     def __init__(self, what, tensors, in_place):
         ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
         if not ts:
             raise L.RtgError(f'{what}: no gradients')
-        for i, t in enumerate(ts):
-            if t.dtype not in _NORM_TYPES or t.layout is not torch.strided:
-                raise L.RtgError(f'{what}: gradient {i} is {t.dtype}, {t.layout} (float32 or bfloat16, strided)')
-            if not t.is_contiguous() and not _dense(t):
-                if in_place:
-                    raise L.RtgError(f'{what}: gradient {i} of shape {tuple(t.shape)} and strides {t.stride()} has gaps or overlaps '
-                                     'itself: it cannot be scaled in place')
-                ts[i] = t.contiguous()
-        _need_here(what, *ts)
+        kinds = list(map(_dtype_of, ts))
+        if not {torch.float32, _BF}.issuperset(kinds):
+            i = next(i for i, k in enumerate(kinds) if k not in _NORM_TYPES)
+            raise L.RtgError(f'{what}: gradient {i} is {kinds[i]} (float32 or bfloat16)')
+        devices = set(map(_TB.get_device, ts))
+        if len(devices) > 1 or devices != {torch.cuda.current_device() if torch.cuda.is_available() else None}:
+            _need_here(what, *ts)
+        if set(map(_layout_of, ts)) != {torch.strided}:
+            raise L.RtgError(f'{what}: sparse gradients')
+        if not all(map(_TB.is_contiguous, ts)):
+            for i, t in enumerate(ts):
+                if not t.is_contiguous() and not _dense(t):
+                    if in_place:
+                        raise L.RtgError(f'{what}: gradient {i} of shape {tuple(t.shape)} and strides {t.stride()} has gaps or '
+                                         'overlaps itself: it cannot be scaled in place')
+                    ts[i] = t.contiguous()
         n = len(ts)
         self.n, self.keep, self.device = n, ts, ts[0].device
-        self.ptrs = (C.c_void_p * n)(*[t.data_ptr() for t in ts])
-        self.counts = (C.c_longlong * n)(*[t.numel() for t in ts])
-        self.bf16 = (C.c_int * n)(*[t.dtype is _BF for t in ts])
+        counts = list(map(_TB.numel, ts))
+        self._arrays = (array.array('Q', map(_TB.data_ptr, ts)), array.array('q', counts), array.array('i', [k is _BF for k in kinds]))
+        self.ptrs, self.counts, self.bf16 = (a.buffer_info()[0] for a in self._arrays)
         self.bytes = sum(t.numel() * t.element_size() for t in ts) if PROFILE is not None else 0
 
     def ws(self):
@@ -1511,8 +1563,8 @@ def total_norm(tensors, norm_type=2.0):
     kind = _norm_kind(norm_type)
     g = _GradList('total_norm', tensors, False)
     ws, out = g.ws(), torch.empty((), device=g.device)
-    check(timed_bw('grad_norm', g.bytes, lambda: lib.rtg_grad_norm(g.n, g.ptrs, g.counts, g.bf16, kind, _p(ws), _p(out), _stream())),
-          'grad_norm')
+    check(timed_bw('grad_norm', g.bytes, lambda: lib.rtg_grad_norm(g.n, g.ptrs, g.counts, g.bf16, kind, ws.data_ptr(), out.data_ptr(),
+                                                                   _stream())), 'grad_norm')
     return out
 
 
@@ -1524,8 +1576,8 @@ def clip_grads_(grads, max_norm, norm_type=2.0):
     kind, limit = _norm_kind(norm_type), _limit(max_norm)
     g = _GradList('clip_grads_', grads, True)
     ws, out = g.ws(), torch.empty((), device=g.device)
-    check(timed_bw('grad_clip', 2 * g.bytes, lambda: lib.rtg_grad_clip(g.n, g.ptrs, g.counts, g.bf16, kind, limit, _p(ws), _p(out),
-                                                                       _stream())), 'grad_clip (do gradients overlap?)')
+    check(timed_bw('grad_clip', 2 * g.bytes, lambda: lib.rtg_grad_clip(g.n, g.ptrs, g.counts, g.bf16, kind, limit, ws.data_ptr(),
+                                                                   out.data_ptr(), _stream())), 'grad_clip (do gradients overlap?)')
     torch.autograd.graph.increment_version(g.keep)
     return out
 
@@ -1545,26 +1597,26 @@ def clipped_adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, max_norm, lr=1e-
         raise L.RtgError(f'clipped_adamw_: lists of {[len(c) for c in cols]} buffers and {len(flags)} loss flags')
     if not grad_scale > 0.0:
         raise L.RtgError(f'clipped_adamw_: grad_scale {grad_scale!r}')
+    every = [t for c in cols for t in c] + [t for t in flags if t is not None] + ([] if out is None else [out])
+    _need_here('clipped_adamw_', *every)
+    if any(t.dtype is not torch.float32 for t in every) or not all(map(_TB.is_contiguous, every)):
+        raise L.RtgError('clipped_adamw_: parameters, gradients, moments, steps and flags have to be contiguous float32 tensors')
     jobs = (L.AdamWJob * n)()
     for i, (p, g, m, v, t) in enumerate(zip(*cols)):
-        _need_here('clipped_adamw_', p, g, m, v, t, flags[i])
-        if any(b.dtype != torch.float32 or not b.is_contiguous() or b.numel() != p.numel() for b in (p, g, m, v)) or p.numel() < 1:
-            raise L.RtgError(f'clipped_adamw_: buffer {i}: parameters, gradients and moments have to be contiguous float32 tensors '
-                             'of one size')
-        if any(b is not None and (b.dtype != torch.float32 or b.numel() != 1) for b in (t, flags[i])):
-            raise L.RtgError(f'clipped_adamw_: buffer {i}: the step and the loss flag have to be float32 scalars on the device')
-        jobs[i] = L.AdamWJob(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), t.data_ptr(),
-                             None if flags[i] is None else flags[i].data_ptr(), p.numel())
+        size, flag = p.numel(), flags[i]
+        if size < 1 or g.numel() != size or m.numel() != size or v.numel() != size:
+            raise L.RtgError(f'clipped_adamw_: buffer {i}: {size} parameters, {g.numel()} gradients, {m.numel()} and {v.numel()} moments')
+        if t.numel() != 1 or (flag is not None and flag.numel() != 1):
+            raise L.RtgError(f'clipped_adamw_: buffer {i}: the step and the loss flag have to be scalars')
+        jobs[i] = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), t.data_ptr(), _ptr(flag), size)
     dev = cols[0][0].device
     if out is None:
         out = torch.empty((), device=dev)
-    else:
-        _need_here('clipped_adamw_', out)
-        if out.dtype != torch.float32 or out.numel() != 1:
-            raise L.RtgError('clipped_adamw_: out has to be a float32 scalar on the device')
+    elif out.numel() != 1:
+        raise L.RtgError('clipped_adamw_: out has to be a scalar')
     ws = torch.empty(lib.rtg_grad_ws(n), device=dev, dtype=torch.float64)
     check(timed_bw('adamw_clipped', 32 * sum(p.numel() for p in cols[0]), lambda: lib.rtg_adamw_clipped(
-        n, jobs, limit, lr, betas[0], betas[1], eps, weight_decay, grad_scale, _p(ws), _p(out), _stream())),
+        n, jobs, limit, lr, betas[0], betas[1], eps, weight_decay, grad_scale, ws.data_ptr(), out.data_ptr(), _stream())),
           'adamw_clipped (do buffers overlap?)')
     torch.autograd.graph.increment_version(cols[0] + cols[2] + cols[3] + cols[4])
     return out
