@@ -14,9 +14,8 @@
 
 namespace {
 
-constexpr int TABLE = 160;            // tensors per launch: the table travels in the kernel's arguments (3.2 KB of 4)
+constexpr int TABLE = 192;            // tensors per launch: the table travels in the kernel's arguments (3.9 KB of 4)
 constexpr int JOBS = 32;              // AdamW buffers per launch
-constexpr int BLOCKS = 2048;          // chunks a list is cut into at least, where it is long: 8 workgroups per CU
 constexpr int THREADS = 256;
 constexpr int REDUCE = 1024;
 
@@ -70,7 +69,15 @@ __device__ __forceinline__ double block_join(double v, double* red) {
 template <int KIND, int N>
 __device__ __forceinline__ double all_partials(const double* __restrict__ part, int n, double* red) {
   double acc = 0.0;
-  for (int i = threadIdx.x; i < n; i += N) acc = join<KIND>(acc, part[i]);
+  int i = threadIdx.x;
+  for (; i + 7 * N < n; i += 8 * N) {                    // (eight loads in flight: one after the other they are microseconds)
+    double v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = part[i + k * N];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc = join<KIND>(acc, v[k]);
+  }
+  for (; i < n; i += N) acc = join<KIND>(acc, part[i]);
   return block_join<KIND, N>(acc, red);
 }
 
@@ -83,11 +90,22 @@ __device__ __forceinline__ float clip_factor(double norm, double max_norm) {
   return f < 1.0 || f != f ? (float)f : 1.f;
 }
 
+// elements in front of the first whole word (a bf16 tensor may start in the middle of one: its vectors would be 4.7 TB/s,
+// those that start with a word 5.7, whatever the line)
+template <class T>
+__device__ __forceinline__ int odd_head(const T* p, long long n) {
+  return sizeof(T) == 2 && n > 0 && (reinterpret_cast<uintptr_t>(p) & 2) ? 1 : 0;
+}
+
 template <class T, int KIND>
 __device__ __forceinline__ double chunk_sum(const T* __restrict__ p, long long n) {
   constexpr int N = RtgVec<T>::N;
-  const long long nv = n / N;
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  const int head = odd_head(p, n);
+  if (head && threadIdx.x == 0) acc[3] = take<KIND>(acc[3], rtg_up(*p));
+  p += head;
+  n -= head;
+  const long long nv = n / N;
   long long i = threadIdx.x;
   for (; i + 3 * THREADS < nv; i += 4 * THREADS) {
     RtgVec<T> v[4];
@@ -142,6 +160,10 @@ __global__ __launch_bounds__(REDUCE) void grad_norm_finish(const double* __restr
 template <class T>
 __device__ __forceinline__ void chunk_scale(T* __restrict__ p, long long n, float f) {
   constexpr int N = RtgVec<T>::N;
+  const int head = odd_head(p, n);
+  if (head && threadIdx.x == 0) rtg_down(rtg_up(*p) * f, *p);
+  p += head;
+  n -= head;
   const long long nv = n / N;
   for (long long i = threadIdx.x; i < nv; i += THREADS) {
     RtgVec<T> v;
@@ -251,10 +273,14 @@ __global__ __launch_bounds__(THREADS) void adam_update(const AdamTable t, const 
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int MAX_TENSORS = 1 << 20;
 
-// bytes of a chunk: about BLOCKS chunks over a long list, at least 16 KB (four rounds of a workgroup's loads)
+// Bytes of a chunk: 2048 chunks (8 workgroups a CU) of 16 to 256 KB each, more of 256 KB where that many do not hold the list
+// (an even end: 1 GB in 2048 chunks 251 us, in 4096 230 us; 110 MB 27 and 28 us), but no more than 8192: the clipping kernels
+// read every partial in every workgroup.
+constexpr int MOST_CHUNKS = 8192;
+long long up(long long bytes) { return (bytes + 4095) / 4096 * 4096; }
 long long chunk_bytes(long long total) {
-  const long long c = (total / BLOCKS + 4095) / 4096 * 4096;
-  return c < 16384 ? 16384 : c;
+  const long long even = up(total / 2048), c = even < 16384 ? 16384 : even > 262144 ? 262144 : even, least = up(total / MOST_CHUNKS);
+  return c > least ? c : least;
 }
 
 // walks the list, TABLE tensors a launch: launch(table, workgroups, workgroups before) for each -> status; *blocks: all of them
@@ -351,8 +377,8 @@ int clip(int n, void* const* grads, const long long* counts, const int* bf16, do
 
 extern "C" long long rtg_grad_ws(int n) {
   if (n < 1 || n > MAX_TENSORS) return RTG_EINVAL;
-  // a partial per chunk (at most BLOCKS full ones and a last one per tensor), and AdamW's scalars
-  return (long long)BLOCKS + n + (long long)n * (sizeof(AdamScalars) / sizeof(double));
+  // a partial per chunk (at most MOST_CHUNKS full ones and a last one per tensor), and AdamW's scalars
+  return (long long)MOST_CHUNKS + n + (long long)n * (sizeof(AdamScalars) / sizeof(double));
 }
 
 extern "C" int rtg_grad_norm(int n, const void* const* grads, const long long* counts, const int* bf16, int kind, double* ws,
@@ -433,9 +459,11 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
     if (rc != RTG_OK) return rc;
     blocks += here;
   }
-  AdamScalars* sc = reinterpret_cast<AdamScalars*>(ws + BLOCKS + n);
+  AdamScalars* sc = reinterpret_cast<AdamScalars*>(ws + MOST_CHUNKS + n);
   AdamTable a;
-  a.chunk = t.chunk / 4;
+  // (smaller pieces than the norm's: four streams in, three out, and no partial a piece: 27 M parameters 172 us, in the norm's 181)
+  const long long piece = up(4 * total / MOST_CHUNKS);
+  a.chunk = (piece < 16384 ? 16384 : piece) / 4;
   for (int i = 0; i < n; i += JOBS) {
     int here = 0;
     for (a.count = 0; a.count < JOBS && i + a.count < n; ++a.count) {

@@ -1518,7 +1518,7 @@ def _limit(max_norm):
 
 
 _TB = torch._C.TensorBase
-_dtype_of, _layout_of = operator.attrgetter('dtype'), operator.attrgetter('layout')
+_dtype_of = operator.attrgetter('dtype')
 
 
 class _GradList:
@@ -1530,25 +1530,29 @@ class _GradList:
         if not ts:
             raise L.RtgError(f'{what}: no gradients')
         kinds = list(map(_dtype_of, ts))
-        if not {torch.float32, _BF}.issuperset(kinds):
+        found = set(kinds)
+        if not found.issubset(_NORM_TYPES):
             i = next(i for i, k in enumerate(kinds) if k not in _NORM_TYPES)
             raise L.RtgError(f'{what}: gradient {i} is {kinds[i]} (float32 or bfloat16)')
-        devices = set(map(_TB.get_device, ts))
-        if len(devices) > 1 or devices != {torch.cuda.current_device() if torch.cuda.is_available() else None}:
+        if set(map(_TB.get_device, ts)) != {torch.cuda.current_device() if torch.cuda.is_available() else None}:
             _need_here(what, *ts)
-        if set(map(_layout_of, ts)) != {torch.strided}:
-            raise L.RtgError(f'{what}: sparse gradients')
-        if not all(map(_TB.is_contiguous, ts)):
-            for i, t in enumerate(ts):
-                if not t.is_contiguous() and not _dense(t):
-                    if in_place:
-                        raise L.RtgError(f'{what}: gradient {i} of shape {tuple(t.shape)} and strides {t.stride()} has gaps or '
-                                         'overlaps itself: it cannot be scaled in place')
-                    ts[i] = t.contiguous()
         n = len(ts)
+        try:
+            if not all(map(_TB.is_contiguous, ts)):
+                for i, t in enumerate(ts):
+                    if not t.is_contiguous() and not _dense(t):
+                        if in_place:
+                            raise L.RtgError(f'{what}: gradient {i} of shape {tuple(t.shape)} and strides {t.stride()} has gaps or '
+                                             'overlaps itself: it cannot be scaled in place')
+                        ts[i] = t.contiguous()
+            ptrs = array.array('Q', map(_TB.data_ptr, ts))
+        except L.RtgError:
+            raise
+        except RuntimeError as e:                               # (sparse gradients have neither strides nor one address)
+            raise L.RtgError(f'{what}: {e}') from None
+        bf16 = array.array('i', [_BF in found] * n if len(found) == 1 else [k is _BF for k in kinds])
         self.n, self.keep, self.device = n, ts, ts[0].device
-        counts = list(map(_TB.numel, ts))
-        self._arrays = (array.array('Q', map(_TB.data_ptr, ts)), array.array('q', counts), array.array('i', [k is _BF for k in kinds]))
+        self._arrays = (ptrs, array.array('q', map(_TB.numel, ts)), bf16)
         self.ptrs, self.counts, self.bf16 = (a.buffer_info()[0] for a in self._arrays)
         self.bytes = sum(t.numel() * t.element_size() for t in ts) if PROFILE is not None else 0
 
