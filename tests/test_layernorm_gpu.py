@@ -13,10 +13,19 @@ KINDS = [torch.float32, torch.bfloat16]
 # (rows, n): single elements, ends inside a vector / a wave / a block, the longest that registers hold and longer ones
 ROWS = [(1, 1), (3, 1), (5, 2), (1, 8), (7, 63), (64, 64), (33, 65), (9, 128), (6, 250), (129, 257), (2, 1000), (4, 1024), (5, 2047),
         (3, 2048), (3, 4096), (3, 4097), (2, 8192), (1, 16384), (2, 16385), (2, 20001), (1, 40000), (1, 70001), (5000, 48), (1500, 512),
-        (700, 1111)]
+        (700, 1111),
+        # rows of less than a vector; several rows a block, whatever its tile
+        (100_003, 3), (4099, 7), (70_000, 24), (2500, 1500), (600, 4096), (530, 9000), (300, 16384), (1100, 12_289), (70, 33_000)]
 # (clips, channels, positions)
 MAPS = [(2, 1, 3), (2, 3, 5), (1, 16, 4), (2, 32, 64), (3, 33, 67), (2, 128, 32), (1, 512, 10), (2, 64, 1025), (1, 1024, 33), (1, 1025, 7),
-        (1, 2500, 70), (2, 2, 4096), (4, 7, 1), (1, 40, 2048), (16, 8, 300), (2, 256, 515), (40, 20, 2), (1, 600, 129)]
+        (1, 2500, 70), (2, 2, 4096), (4, 7, 1), (1, 40, 2048), (16, 8, 300), (2, 256, 515), (40, 20, 2), (1, 600, 129),
+        # clips of less than a vector of positions
+        (3, 40, 2), (2, 33, 3), (5, 128, 7), (300, 500, 5), (2, 1000, 6), (50, 1024, 4), (1, 2000, 3),
+        # no more than two vectors of positions, each cut of the channels
+        (9, 100, 8), (7, 250, 11), (5, 500, 16), (3, 1024, 9),
+        # every tile for maps that fill the chip, several tiles a block
+        (70, 5, 9001), (40, 13, 8200), (33, 30, 8001), (32, 61, 4101), (17, 100, 8003), (9, 200, 8003), (5, 400, 7001), (3, 1000, 5003),
+        (3, 1100, 500), (2, 2048, 11), (4, 2049, 130)]
 
 
 def make(shape, kind, seed, level=1.0):

@@ -9,7 +9,7 @@
 
 namespace {
 
-constexpr int LOOP_THREADS = 256;
+constexpr int LOOP_THREADS = 1024;
 constexpr int FIN_COLS = 32, FIN_ROWS = 32;
 
 struct LnShape {
@@ -47,6 +47,8 @@ __device__ __forceinline__ void load_params(float (&out)[N], const void* p, int 
     const rtg_bf16* q = reinterpret_cast<const rtg_bf16*>(p) + i;
 #pragma unroll
     for (int e = 0; e < N; ++e) out[e] = rtg_up(q[e]);
+  } else if constexpr (N == 1) {
+    out[0] = reinterpret_cast<const float*>(p)[i];
   } else {
 #pragma unroll
     for (int k = 0; k < N / 4; ++k) {
@@ -60,6 +62,7 @@ __device__ __forceinline__ void load_params(float (&out)[N], const void* p, int 
 
 template <int N>
 __device__ __forceinline__ void store_floats(const float (&v)[N], float* p) {
+  if constexpr (N == 1) *p = v[0];
 #pragma unroll
   for (int k = 0; k < N / 4; ++k) {
     RtgVec<float> r;
@@ -348,17 +351,18 @@ __device__ __forceinline__ void tile_sum(float (&v)[K], float (*red)[64 * rtg_sc
 
 constexpr int map_teams(int w) { return w < 4 ? 4 / w : 1; }
 constexpr int map_block(int w) { return 64 * w * map_teams(w); }
-template <class T, int LP, int W, int CPT>
+template <class V, int LP, int W, int CPT>
 struct MapTile {
-  static constexpr int N = RtgVec<T>::N, CL = 64 / LP, TEAMS = map_teams(W), BLK = map_block(W);
+  static constexpr int N = V::N, CL = 64 / LP, TEAMS = map_teams(W), BLK = map_block(W);
   static constexpr int POS = LP * N, CH = CL * W * CPT;
 };
 
 // where a lane of a tile stands.  The wave's part of every address is scalar, a lane's is 32 bits; a lane without a channel
 // works on channel lane 0's (of the last channel, where the wave has none) for nothing
-template <class T, int LP, int W, int CPT>
+template <class V, int LP, int W, int CPT>
 struct MapLane {
-  using M = MapTile<T, LP, W, CPT>;
+  using T = typename V::T;
+  using M = MapTile<V, LP, W, CPT>;
   int lane, wave, cw, n;                 // cw: the wave's first channel
   bool full;                             // every lane of the wave has CPT channels
   unsigned o, t;                         // clip, first position of the lane's vector
@@ -385,7 +389,7 @@ struct MapLane {
   __device__ __forceinline__ static const T* byte(const T* p, unsigned off) {
     return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + off);
   }
-  __device__ __forceinline__ void load(RtgVec<T> (&v)[CPT], const T* p, long long outer, long long stride) const {
+  __device__ __forceinline__ void load(V (&v)[CPT], const T* p, long long outer, long long stride) const {
     p += o * outer;
     if (full) {
 #pragma unroll
@@ -426,18 +430,18 @@ struct MapLane {
   }
 };
 
-template <class T, int LP, int W, int CPT>
+template <class V, int LP, int W, int CPT, class T = typename V::T>
 __global__ __launch_bounds__(map_block(W)) void ln_map_fwd(LnShape s, const T* __restrict__ x, const void* __restrict__ w,
                                                                            const void* __restrict__ b, T* __restrict__ y,
                                                                            float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  using M = MapTile<T, LP, W, CPT>;
+  using M = MapTile<V, LP, W, CPT>;
   constexpr int N = M::N;
   constexpr int R = rtg_scattered(LP, N);
   __shared__ float red[2][W > 1 ? M::BLK / 64 : 1][64 * R];
-  MapLane<T, LP, W, CPT> at(s);
+  MapLane<V, LP, W, CPT> at(s);
   const unsigned per = (unsigned)((s.inner + M::POS - 1) / M::POS);
   at.go(s, xcd_order(blockIdx.x, gridDim.x) * M::TEAMS + at.wave / W, (unsigned)s.outer * per, per);
-  RtgVec<T> v[CPT];
+  V v[CPT];
   at.load(v, x, s.xo, s.xn);
   float wr[CPT], br[CPT], a[N], mean[N], rstd[N];
   at.params(wr, w, s.pbf, 1.f);
@@ -486,17 +490,17 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_fwd(LnShape s, const T* _
 
 // dx and the team's share of dw, db: a lane adds its channels' products over its positions and over the tiles its team walks;
 // the position lanes meet in shuffles at the end, the teams of a block in LDS
-template <class T, int LP, int W, int CPT>
+template <class V, int LP, int W, int CPT, class T = typename V::T>
 __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* __restrict__ dy, const T* __restrict__ x,
                                                                            const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                                                                            const void* __restrict__ w, T* __restrict__ dx,
                                                                            float* __restrict__ part) {
-  using M = MapTile<T, LP, W, CPT>;
+  using M = MapTile<V, LP, W, CPT>;
   constexpr int N = M::N;
   constexpr int R = rtg_scattered(LP, 2 * N);
   __shared__ float red[2][W > 1 ? M::BLK / 64 : 1][64 * R];
   __shared__ float sums[2][M::TEAMS][M::CH];
-  MapLane<T, LP, W, CPT> at(s);
+  MapLane<V, LP, W, CPT> at(s);
   const int team = at.wave / W;
   const unsigned per = (unsigned)((s.inner + M::POS - 1) / M::POS), tiles = (unsigned)s.outer * per;
   float wr[CPT], aw[CPT], ab[CPT];
@@ -506,7 +510,7 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* _
   int turn = 0;
   for (unsigned base = xcd_order(blockIdx.x, gridDim.x) * M::TEAMS; base < tiles; base += gridDim.x * M::TEAMS, turn ^= 1) {
     at.go(s, base + team, tiles, per);
-    RtgVec<T> xv[CPT], gv[CPT];
+    V xv[CPT], gv[CPT];
     at.load(xv, x, s.xo, s.xn);
     at.load(gv, dy, s.n * s.inner, s.inner);
     float mean[N], rstd[N], a[2 * N];
@@ -568,26 +572,85 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* _
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Kernels for any size.  A row that no register kernel holds is read once per sum; the later reads come from L2.
+// Kernels for any size.  A row or a column of channels that no register kernel holds is read once per sum (the later reads
+// come from L2 or the memory-side cache): 1000 rows of 40000.  They also serve rows of less than a vector, a thread each.
 // ---------------------------------------------------------------------------------------------------------------------
+template <int BLK>
+__device__ __forceinline__ float loop_sum(float v, float* red) {
+  v = rtg_group_sum<64>(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < BLK / 64; ++i) v += red[i];
+  return v;
+}
+
+// f(first element, vector of x, vector of g) for the whole vectors of a row, f(element, x, g) for those behind them; x or g alone
+// where the other is the same pointer
+template <class T, class F>
+__device__ __forceinline__ void row_walk(const T* x, const T* g, long long n, F f) {
+  constexpr int N = RtgVec<T>::N;
+  const long long nv = n / N;
+#pragma unroll 2
+  for (long long i = threadIdx.x; i < nv; i += LOOP_THREADS) {
+    RtgVec<T> a, b;
+    a.load(x + i * N);
+    b.load(g + i * N);
+    float xv[N], gv[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      xv[e] = a.get(e);
+      gv[e] = b.get(e);
+    }
+    f(i * N, xv, gv);
+  }
+  if (nv * N + threadIdx.x < n) {
+    const float xv[1] = {rtg_up(x[nv * N + threadIdx.x])}, gv[1] = {rtg_up(g[nv * N + threadIdx.x])};
+    f(nv * N + threadIdx.x, xv, gv);
+  }
+}
+template <class T, int K>
+__device__ __forceinline__ void put_row(const float (&v)[K], T* p) {
+  if constexpr (K == 1) {
+    rtg_down(v[0], *p);
+  } else {
+    RtgVec<T> r;
+    r.set(v);
+    r.store(p);
+  }
+}
+
 template <class T>
 __global__ __launch_bounds__(LOOP_THREADS) void ln_row_loop_fwd(LnShape s, const T* __restrict__ x, const void* __restrict__ w,
                                                                 const void* __restrict__ b, T* __restrict__ y,
                                                                 float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  __shared__ float red[4];
+  __shared__ float red[LOOP_THREADS / 64];
   for (long long row = blockIdx.x; row < s.outer; row += gridDim.x) {
     const T* xr = x + row * s.xo;
+    T* yr = y + row * s.n;
     float acc = 0.f;
-    for (long long i = threadIdx.x; i < s.n; i += LOOP_THREADS) acc += rtg_up(xr[i]);
-    const float mean = mean_of(rtg_block_sum(acc, red), s);
+    row_walk(xr, xr, s.n, [&](long long, auto& v, auto&) __attribute__((always_inline)) {
+#pragma unroll
+      for (float e : v) acc += e;
+    });
+    const float mean = mean_of(loop_sum<LOOP_THREADS>(acc, red), s);
     acc = 0.f;
-    for (long long i = threadIdx.x; i < s.n; i += LOOP_THREADS) {
-      const float d = rtg_up(xr[i]) - mean;
-      acc += d * d;
-    }
-    const float rstd = rstd_of(rtg_block_sum(acc, red), s);
-    for (long long i = threadIdx.x; i < s.n; i += LOOP_THREADS)
-      rtg_down((rtg_up(xr[i]) - mean) * rstd * param_at(w, s.pbf, i, 1.f) + param_at(b, s.pbf, i, 0.f), y[row * s.n + i]);
+    row_walk(xr, xr, s.n, [&](long long, auto& v, auto&) __attribute__((always_inline)) {
+#pragma unroll
+      for (float e : v) acc += (e - mean) * (e - mean);
+    });
+    const float rstd = rstd_of(loop_sum<LOOP_THREADS>(acc, red), s);
+    row_walk(xr, xr, s.n, [&](long long i, auto& v, auto&) __attribute__((always_inline)) {
+      constexpr int K = sizeof(v) / sizeof(float);
+      float wr[K], br[K], o[K];
+      load_params<K>(wr, w, s.pbf, i, 1.f);
+      load_params<K>(br, b, s.pbf, i, 0.f);
+#pragma unroll
+      for (int e = 0; e < K; ++e) o[e] = (v[e] - mean) * rstd * wr[e] + br[e];
+      put_row(o, yr + i);
+    });
     if (mean_out && threadIdx.x == 0) {
       mean_out[row] = mean;
       rstd_out[row] = rstd;
@@ -599,62 +662,169 @@ template <class T>
 __global__ __launch_bounds__(LOOP_THREADS) void ln_row_loop_dx(LnShape s, const T* __restrict__ dy, const T* __restrict__ x,
                                                                const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                                                                const void* __restrict__ w, T* __restrict__ dx) {
-  __shared__ float red[4];
+  __shared__ float red[LOOP_THREADS / 64];
   for (long long row = blockIdx.x; row < s.outer; row += gridDim.x) {
     const T *xr = x + row * s.xo, *gr = dy + row * s.n;
     const float mean = mean_in[row], rstd = rstd_in[row];
     float a1 = 0.f, a2 = 0.f;
-    for (long long i = threadIdx.x; i < s.n; i += LOOP_THREADS) {
-      const float g = rtg_up(gr[i]) * param_at(w, s.pbf, i, 1.f);
-      a1 += g;
-      a2 += g * ((rtg_up(xr[i]) - mean) * rstd);
-    }
-    const float c1 = rtg_block_sum(a1, red) * s.inv_n, c2 = rtg_block_sum(a2, red) * s.inv_n;
-    for (long long i = threadIdx.x; i < s.n; i += LOOP_THREADS) {
-      const float g = rtg_up(gr[i]) * param_at(w, s.pbf, i, 1.f);
-      rtg_down(rstd * (g - c1 - (rtg_up(xr[i]) - mean) * rstd * c2), dx[row * s.n + i]);
-    }
+    row_walk(xr, gr, s.n, [&](long long i, auto& v, auto& d) __attribute__((always_inline)) {
+      constexpr int K = sizeof(v) / sizeof(float);
+      float wr[K];
+      load_params<K>(wr, w, s.pbf, i, 1.f);
+#pragma unroll
+      for (int e = 0; e < K; ++e) {
+        a1 += d[e] * wr[e];
+        a2 += d[e] * wr[e] * ((v[e] - mean) * rstd);
+      }
+    });
+    const float c1 = loop_sum<LOOP_THREADS>(a1, red) * s.inv_n, c2 = loop_sum<LOOP_THREADS>(a2, red) * s.inv_n;
+    row_walk(xr, gr, s.n, [&](long long i, auto& v, auto& d) __attribute__((always_inline)) {
+      constexpr int K = sizeof(v) / sizeof(float);
+      float wr[K], o[K];
+      load_params<K>(wr, w, s.pbf, i, 1.f);
+#pragma unroll
+      for (int e = 0; e < K; ++e) o[e] = rstd * (d[e] * wr[e] - c1 - (v[e] - mean) * rstd * c2);
+      put_row(o, dx + row * s.n + i);
+    });
   }
 }
 
-// partial dw, db of slice blockIdx.y of the rows: 64 adjacent columns a block, its four waves every fourth row
+// partial dw, db of slice blockIdx.y of the rows: a vector of columns a lane, the block's sixteen waves every sixteenth row
+constexpr int DW_WAVES = LOOP_THREADS / 64;
 template <class T>
 __global__ __launch_bounds__(LOOP_THREADS) void ln_row_loop_dw(LnShape s, const T* __restrict__ dy, const T* __restrict__ x,
                                                                const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                float* __restrict__ part, int slices) {
-  __shared__ float red[2][4][64];
+  constexpr int N = RtgVec<T>::N;
+  __shared__ float red[DW_WAVES][64 * N];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long i = (long long)blockIdx.x * 64 + lane;
-  float aw = 0.f, ab = 0.f;
-  if (i < s.n)
-    for (long long row = blockIdx.y * 4 + wave; row < s.outer; row += 4 * slices) {
-      const float g = rtg_up(dy[row * s.n + i]);
-      aw += g * ((rtg_up(x[row * s.xo + i]) - mean[row]) * rstd[row]);
-      ab += g;
+  const long long i = ((long long)blockIdx.x * 64 + lane) * N, at = i < s.n - N ? i : s.n - N;      // (n >= N: ln_tiny has the rest)
+  float aw[N], ab[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) aw[e] = ab[e] = 0.f;
+  for (long long row = blockIdx.y * DW_WAVES + wave; row < s.outer; row += (long long)DW_WAVES * slices) {
+    RtgVec<T> xv, gv;
+    xv.load(x + row * s.xo + at);
+    gv.load(dy + row * s.n + at);
+    const float m = mean[row], r = rstd[row];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      aw[e] += gv.get(e) * ((xv.get(e) - m) * r);
+      ab[e] += gv.get(e);
     }
-  red[0][wave][lane] = aw;
-  red[1][wave][lane] = ab;
-  __syncthreads();
-  if (wave < 2 && i < s.n)
-    part[((long long)blockIdx.y * 2 + wave) * s.n + i] =
-        (red[wave][0][lane] + red[wave][1][lane]) + (red[wave][2][lane] + red[wave][3][lane]);
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < N; ++e) red[wave][lane * N + e] = which ? ab[e] : aw[e];
+    __syncthreads();
+    for (int j = threadIdx.x; j < 64 * N; j += LOOP_THREADS) {
+      const long long first = ((long long)blockIdx.x * 64 + j / N) * N, col = first < s.n - N ? first : s.n - N;
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < DW_WAVES; ++k) v += red[k][j];
+      if (j % N >= first - col) part[((long long)blockIdx.y * 2 + which) * s.n + col + j % N] = v;
+    }
+  }
 }
 
-// the sum over a block's four waves of `v` at each lane, in every wave
-__device__ __forceinline__ float wave_column_sum(float v, float (&red)[4][64]) {
+// rows of less than a vector (n < 8): a thread a row
+constexpr int TINY_THREADS = 256, TINY_MOST = 7;
+template <class T>
+__global__ __launch_bounds__(TINY_THREADS) void ln_tiny_fwd(LnShape s, const T* __restrict__ x, const void* __restrict__ w,
+                                                            const void* __restrict__ b, T* __restrict__ y, float* __restrict__ mean_out,
+                                                            float* __restrict__ rstd_out) {
+  const int n = (int)s.n;
+  for (long long row = (long long)blockIdx.x * TINY_THREADS + threadIdx.x; row < s.outer; row += (long long)gridDim.x * TINY_THREADS) {
+    float v[TINY_MOST], sum = 0.f, sq = 0.f;
+#pragma unroll
+    for (int e = 0; e < TINY_MOST; ++e) {
+      v[e] = e < n ? rtg_up(x[row * s.xo + e]) : 0.f;
+      sum += v[e];
+    }
+    const float mean = mean_of(sum, s);
+#pragma unroll
+    for (int e = 0; e < TINY_MOST; ++e) sq += e < n ? (v[e] - mean) * (v[e] - mean) : 0.f;
+    const float rstd = rstd_of(sq, s);
+#pragma unroll
+    for (int e = 0; e < TINY_MOST; ++e)
+      if (e < n) rtg_down((v[e] - mean) * rstd * param_at(w, s.pbf, e, 1.f) + param_at(b, s.pbf, e, 0.f), y[row * n + e]);
+    if (mean_out) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(TINY_THREADS) void ln_tiny_bwd(LnShape s, const T* __restrict__ dy, const T* __restrict__ x,
+                                                            const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                                                            const void* __restrict__ w, T* __restrict__ dx, float* __restrict__ part) {
+  __shared__ float red[TINY_THREADS / 64][2 * TINY_MOST];
+  const int n = (int)s.n;
+  float aw[TINY_MOST], ab[TINY_MOST], wr[TINY_MOST];
+#pragma unroll
+  for (int e = 0; e < TINY_MOST; ++e) {
+    aw[e] = ab[e] = 0.f;
+    wr[e] = e < n ? param_at(w, s.pbf, e, 1.f) : 0.f;
+  }
+  for (long long row = (long long)blockIdx.x * TINY_THREADS + threadIdx.x; row < s.outer; row += (long long)gridDim.x * TINY_THREADS) {
+    const float mean = mean_in[row], rstd = rstd_in[row];
+    float d[TINY_MOST], h[TINY_MOST], a1 = 0.f, a2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < TINY_MOST; ++e) {
+      d[e] = e < n ? rtg_up(dy[row * n + e]) : 0.f;
+      h[e] = e < n ? (rtg_up(x[row * s.xo + e]) - mean) * rstd : 0.f;
+      aw[e] += d[e] * h[e];
+      ab[e] += d[e];
+      a1 += d[e] * wr[e];
+      a2 += d[e] * wr[e] * h[e];
+    }
+    if (!dx) continue;
+    const float c1 = a1 * s.inv_n, c2 = a2 * s.inv_n;
+#pragma unroll
+    for (int e = 0; e < TINY_MOST; ++e)
+      if (e < n) rtg_down(rstd * (d[e] * wr[e] - c1 - h[e] * c2), dx[row * n + e]);
+  }
+  if (!part) return;
+#pragma unroll
+  for (int e = 0; e < TINY_MOST; ++e) {
+    const float a = rtg_group_sum<64>(aw[e]), b = rtg_group_sum<64>(ab[e]);
+    if ((threadIdx.x & 63) == 0) {
+      red[threadIdx.x >> 6][e] = a;
+      red[threadIdx.x >> 6][TINY_MOST + e] = b;
+    }
+  }
+  __syncthreads();
+  const int which = threadIdx.x / 8, e = threadIdx.x % 8;
+  if (which < 2 && e < n) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < TINY_THREADS / 64; ++k) v += red[k][which * TINY_MOST + e];
+    part[((long long)blockIdx.x * 2 + which) * n + e] = v;
+  }
+}
+
+// the sum over a block's waves of `v` at each lane, in every wave
+__device__ __forceinline__ float wave_column_sum(float v, float (&red)[LOOP_THREADS / 64][64]) {
   const int lane = threadIdx.x & 63;
   __syncthreads();
   red[threadIdx.x >> 6][lane] = v;
   __syncthreads();
-  return (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < LOOP_THREADS / 64; ++i) v += red[i][lane];
+  return v;
 }
 
-// feature maps: a lane is a position, the four waves share the channels
+// feature maps: a lane is a position, the waves share the channels
+constexpr int MAP_WAVES = LOOP_THREADS / 64;
 template <class T>
 __global__ __launch_bounds__(LOOP_THREADS) void ln_map_loop_fwd(LnShape s, const T* __restrict__ x, const void* __restrict__ w,
                                                                 const void* __restrict__ b, T* __restrict__ y,
                                                                 float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  __shared__ float red[4][64];
+  __shared__ float red[MAP_WAVES][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long tiles = (s.inner + 63) / 64;
   for (long long tile = blockIdx.x; tile < s.outer * tiles; tile += gridDim.x) {
@@ -663,18 +833,21 @@ __global__ __launch_bounds__(LOOP_THREADS) void ln_map_loop_fwd(LnShape s, const
     const T* xp = x + o * s.xo + t;
     float acc = 0.f;
     if (in)
-      for (long long c = wave; c < s.n; c += 4) acc += rtg_up(xp[c * s.xn]);
+#pragma unroll 4
+      for (long long c = wave; c < s.n; c += MAP_WAVES) acc += rtg_up(xp[c * s.xn]);
     const float mean = mean_of(wave_column_sum(acc, red), s);
     acc = 0.f;
     if (in)
-      for (long long c = wave; c < s.n; c += 4) {
+#pragma unroll 4
+      for (long long c = wave; c < s.n; c += MAP_WAVES) {
         const float d = rtg_up(xp[c * s.xn]) - mean;
         acc += d * d;
       }
     const float rstd = rstd_of(wave_column_sum(acc, red), s);
     if (!in) continue;
     T* yp = y + o * s.n * s.inner + t;
-    for (long long c = wave; c < s.n; c += 4)
+#pragma unroll 4
+    for (long long c = wave; c < s.n; c += MAP_WAVES)
       rtg_down((rtg_up(xp[c * s.xn]) - mean) * rstd * param_at(w, s.pbf, c, 1.f) + param_at(b, s.pbf, c, 0.f), yp[c * s.inner]);
     if (mean_out && wave == 0) {
       mean_out[o * s.inner + t] = mean;
@@ -687,7 +860,7 @@ template <class T>
 __global__ __launch_bounds__(LOOP_THREADS) void ln_map_loop_dx(LnShape s, const T* __restrict__ dy, const T* __restrict__ x,
                                                                const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
                                                                const void* __restrict__ w, T* __restrict__ dx) {
-  __shared__ float red[4][64];
+  __shared__ float red[MAP_WAVES][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long tiles = (s.inner + 63) / 64;
   for (long long tile = blockIdx.x; tile < s.outer * tiles; tile += gridDim.x) {
@@ -698,7 +871,8 @@ __global__ __launch_bounds__(LOOP_THREADS) void ln_map_loop_dx(LnShape s, const 
     if (in) {
       mean = mean_in[o * s.inner + t];
       rstd = rstd_in[o * s.inner + t];
-      for (long long c = wave; c < s.n; c += 4) {
+#pragma unroll 4
+      for (long long c = wave; c < s.n; c += MAP_WAVES) {
         const float g = rtg_up(gp[c * s.inner]) * param_at(w, s.pbf, c, 1.f);
         a1 += g;
         a2 += g * ((rtg_up(xp[c * s.xn]) - mean) * rstd);
@@ -707,30 +881,32 @@ __global__ __launch_bounds__(LOOP_THREADS) void ln_map_loop_dx(LnShape s, const 
     const float c1 = wave_column_sum(a1, red) * s.inv_n, c2 = wave_column_sum(a2, red) * s.inv_n;
     if (!in) continue;
     T* dp = dx + o * s.n * s.inner + t;
-    for (long long c = wave; c < s.n; c += 4) {
+#pragma unroll 4
+    for (long long c = wave; c < s.n; c += MAP_WAVES) {
       const float g = rtg_up(gp[c * s.inner]) * param_at(w, s.pbf, c, 1.f);
       rtg_down(rstd * (g - c1 - (rtg_up(xp[c * s.xn]) - mean) * rstd * c2), dp[c * s.inner]);
     }
   }
 }
 
-// partial dw, db of one channel (blockIdx.x) over slice blockIdx.y of the positions of all clips
+// partial dw, db of one channel (blockIdx.x) over slice blockIdx.y of the clips: adjacent positions in adjacent threads
 template <class T>
-__global__ __launch_bounds__(LOOP_THREADS) void ln_map_loop_dw(LnShape s, const T* __restrict__ dy, const T* __restrict__ x,
+__global__ __launch_bounds__(TINY_THREADS) void ln_map_loop_dw(LnShape s, const T* __restrict__ dy, const T* __restrict__ x,
                                                                const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                float* __restrict__ part, int slices) {
-  __shared__ float red[4];
+  __shared__ float red[TINY_THREADS / 64];
   const long long total = s.outer * s.inner;
   for (long long c = blockIdx.x; c < s.n; c += gridDim.x) {
     float aw = 0.f, ab = 0.f;
-    for (long long p = (long long)blockIdx.y * LOOP_THREADS + threadIdx.x; p < total; p += (long long)slices * LOOP_THREADS) {
+#pragma unroll 4
+    for (long long p = (long long)blockIdx.y * TINY_THREADS + threadIdx.x; p < total; p += (long long)slices * TINY_THREADS) {
       const long long o = p / s.inner, t = p - o * s.inner;
       const float g = rtg_up(dy[(o * s.n + c) * s.inner + t]);
       aw += g * ((rtg_up(x[o * s.xo + c * s.xn + t]) - mean[p]) * rstd[p]);
       ab += g;
     }
-    aw = rtg_block_sum(aw, red);
-    ab = rtg_block_sum(ab, red);
+    aw = loop_sum<TINY_THREADS>(aw, red);
+    ab = loop_sum<TINY_THREADS>(ab, red);
     if (threadIdx.x == 0) {
       part[((long long)blockIdx.y * 2) * s.n + c] = aw;
       part[((long long)blockIdx.y * 2 + 1) * s.n + c] = ab;
@@ -795,7 +971,7 @@ bool is_rows(const RtgLayerNormDesc* d) { return d->inner == 1; }
 // What serves a problem: the smallest register tile that holds the normalised axis, else the kernels for any size.  `tile` is
 // the tile's number in the dispatch below, `blocks` the grid, in the backward also the number of partial dw / db.
 struct Plan { int tile; int blocks; };
-constexpr int LOOPS = -1;
+constexpr int LOOPS = -1, TINY = -2;
 
 // Rows: threads per row, 16-byte vectors per thread, threads per block.  Over 13 widths from 64 to 16384 and row counts from 1 to
 // 65536 these tiles are within 5 % of the best of 20 (forward) and 40 (backward); what they weigh: a wave's rows need no
@@ -813,7 +989,7 @@ constexpr RowTile BWD_BF16[ROW_TILES] = {{8, 1, 512},   {16, 1, 512},  {32, 1, 5
 
 int row_tile(const RowTile* tiles, long long n, int bf16) {
   const int vec = bf16 ? 8 : 4;
-  if (n < vec) return LOOPS;
+  if (n < vec) return TINY;
   const long long nv = (n + vec - 1) / vec;
   for (int i = 0; i < ROW_TILES; ++i)
     if (nv <= tiles[i].tpr * tiles[i].vpt) return i;
@@ -828,25 +1004,38 @@ int row_tile(const RowTile* tiles, long long n, int bf16) {
 //     chip twice: 128 channels x 65536 positions 13.5 us against 17.4 with four channels a lane and four waves; with 1024
 //     positions it is the other way round, 4.6 against 3.6: more waves, fewer loads each;
 //   - two position lanes where a clip has no more than two vectors of positions (512 channels x 8: 3.7 us against 4.2).
-constexpr int map_key(int lp, int w, int cpt) { return lp * 10000 + w * 100 + cpt; }
+//   - single elements in the place of vectors where a clip has fewer positions than a vector.
+constexpr int map_key(int lp, int w, int cpt, bool one = false) { return (one ? 1000000 : 0) + lp * 10000 + w * 100 + cpt; }
 #define LN_MAP_FWD(X) \
   X(16, 1, 2) X(16, 1, 4) X(8, 1, 4) X(8, 2, 4) X(8, 4, 4) X(4, 4, 4) X(4, 8, 4) X(2, 1, 4) X(2, 2, 4) X(2, 4, 4) X(2, 8, 4) \
-  X(8, 1, 8) X(8, 1, 16) X(8, 2, 16) X(8, 4, 16) X(8, 8, 16)
+  X(8, 1, 8) X(8, 1, 16) X(8, 2, 16) X(8, 4, 16) X(8, 8, 16) X(4, 16, 8)
 #define LN_MAP_BWD(X) \
   X(16, 1, 2) X(16, 1, 4) X(8, 1, 4) X(8, 2, 4) X(8, 4, 4) X(8, 8, 4) X(4, 4, 4) X(4, 8, 4) X(2, 1, 4) X(2, 2, 4) X(2, 4, 4) X(2, 8, 4) \
-  X(8, 2, 8) X(8, 8, 8) X(4, 8, 8)
+  X(8, 2, 8) X(8, 8, 8) X(4, 8, 8) X(2, 16, 4)
+#define LN_MAP_ONE(X) X(8, 1, 4) X(8, 4, 4) X(8, 8, 8) X(8, 8, 16)
 
+#define LN_MAP(LP, W, CPT) LN_MAP_CASE(RtgVec<T>, false, LP, W, CPT)
+#define LN_MAP1(LP, W, CPT) LN_MAP_CASE(RtgOne<T>, true, LP, W, CPT)
+
+bool map_one(const RtgLayerNormDesc* d) { return d->inner < (d->bf16 ? 8 : 4); }
 long long map_tiles(const RtgLayerNormDesc* d, int lp) {
-  const long long pos = lp * (d->bf16 ? 8 : 4);
+  const long long pos = lp * (map_one(d) ? 1 : d->bf16 ? 8 : 4);
   return d->outer * ((d->inner + pos - 1) / pos);
+}
+// (two vectors of positions a clip at most)
+int map_short_key(long long n) {
+  return n <= 128 ? map_key(2, 1, 4) : n <= 256 ? map_key(2, 2, 4) : n <= 512 ? map_key(2, 4, 4) : map_key(2, 8, 4);
+}
+int map_one_key(long long n) {
+  return n <= 32 ? map_key(8, 1, 4, true) : n <= 128 ? map_key(8, 4, 4, true) : n <= 512 ? map_key(8, 8, 8, true) : map_key(8, 8, 16, true);
 }
 // two of a wide tile's waves for every SIMD (256 CUs of four)
 bool map_wide(const RtgLayerNormDesc* d, int lp, int w) { return map_tiles(d, lp) * w >= 2048; }
 
 int map_fwd(const RtgLayerNormDesc* d) {
   const long long n = d->n;
-  if (d->inner <= (d->bf16 ? 16 : 8))
-    return n <= 128 ? map_key(2, 1, 4) : n <= 256 ? map_key(2, 2, 4) : n <= 512 ? map_key(2, 4, 4) : map_key(2, 8, 4);
+  if (map_one(d)) return map_one_key(n);
+  if (d->inner <= (d->bf16 ? 16 : 8) && n <= 1024) return map_short_key(n);
   if (n <= 8) return map_key(16, 1, 2);
   if (n <= 16) return map_key(16, 1, 4);
   if (n <= 32) return map_key(8, 1, 4);
@@ -854,13 +1043,14 @@ int map_fwd(const RtgLayerNormDesc* d) {
   if (n <= 128) return map_wide(d, 8, 1) ? map_key(8, 1, 16) : map_key(8, 4, 4);
   if (n <= 256) return map_wide(d, 8, 2) ? map_key(8, 2, 16) : map_key(4, 4, 4);
   if (n <= 512) return map_wide(d, 8, 4) ? map_key(8, 4, 16) : map_tiles(d, 8) >= 64 ? map_key(4, 8, 4) : map_key(2, 4, 4);
-  return map_wide(d, 8, 8) ? map_key(8, 8, 16) : map_key(2, 8, 4);
+  if (n <= 1024) return map_wide(d, 8, 8) ? map_key(8, 8, 16) : map_key(2, 8, 4);
+  return map_key(4, 16, 8);
 }
 
 int map_bwd(const RtgLayerNormDesc* d) {
   const long long n = d->n;
-  if (d->inner <= (d->bf16 ? 16 : 8))
-    return n <= 128 ? map_key(2, 1, 4) : n <= 256 ? map_key(2, 2, 4) : n <= 512 ? map_key(2, 4, 4) : map_key(2, 8, 4);
+  if (map_one(d)) return map_one_key(n);
+  if (d->inner <= (d->bf16 ? 16 : 8) && n <= 1024) return map_short_key(n);
   if (n <= 8) return map_key(16, 1, 2);
   if (n <= 16) return map_key(16, 1, 4);
   if (n <= 32) return map_key(8, 1, 4);
@@ -868,14 +1058,15 @@ int map_bwd(const RtgLayerNormDesc* d) {
   if (n <= 128) return map_wide(d, 8, 1) ? map_key(8, 2, 8) : map_key(8, 4, 4);
   if (n <= 256) return map_wide(d, 8, 8) ? map_key(8, 8, 4) : map_key(4, 4, 4);
   if (n <= 512) return map_wide(d, 8, 2) ? map_key(8, 8, 8) : map_key(4, 8, 4);
-  return map_wide(d, 4, 8) ? map_key(4, 8, 8) : map_key(2, 8, 4);
+  if (n <= 1024) return map_wide(d, 4, 8) ? map_key(4, 8, 8) : map_key(2, 8, 4);
+  return map_key(2, 16, 4);
 }
 
 // blocks that give each team one tile; 0: no register tile holds the problem (or a lane's offset in a tile would pass 32 bits)
 long long map_blocks(const RtgLayerNormDesc* d, int key) {
-  const int channels = 64 / (key / 10000) * (key / 100 % 100) * (key % 100);
-  if (d->inner < (d->bf16 ? 8 : 4) || d->n > channels || d->inner >= 1 << 24 || d->x_n >= 1 << 24) return 0;
-  const long long tiles = map_tiles(d, key / 10000), teams = map_teams(key / 100 % 100);
+  const int lp = key / 10000 % 100, w = key / 100 % 100, cpt = key % 100;
+  if (d->n > 64 / lp * w * cpt || d->inner >= 1 << 24 || d->x_n >= 1 << 24) return 0;
+  const long long tiles = map_tiles(d, lp), teams = map_teams(w);
   return tiles >= 1ll << 30 ? 0 : (tiles + teams - 1) / teams;
 }
 
@@ -889,6 +1080,7 @@ Plan plan_fwd(const RtgLayerNormDesc* d) {
   if (is_rows(d)) {
     const int i = row_tile(FWD_TILES, d->n, d->bf16);
     if (i == LOOPS) return {LOOPS, (int)lmin(d->outer, 1 << 20)};
+    if (i == TINY) return {TINY, even_blocks((d->outer + TINY_THREADS - 1) / TINY_THREADS, 2048)};
     const int groups = FWD_TILES[i].blk / FWD_TILES[i].tpr;
     return {i, even_blocks((d->outer + groups - 1) / groups, 256 * (1024 / FWD_TILES[i].blk))};
   }
@@ -902,15 +1094,17 @@ Plan plan_bwd(const RtgLayerNormDesc* d) {
   if (is_rows(d)) {
     const RowTile* tiles = d->bf16 ? BWD_BF16 : BWD_F32;
     const int i = row_tile(tiles, d->n, d->bf16);
-    if (i != LOOPS) {
-      // 256 blocks: two partials a CU would be more to add than the second block gains.  One block alone writes dw and db
-      // itself; it is worth that for a few rounds of rows (16 x 512: 4.4 us, in two blocks and ln_finish 5.7).
-      const int groups = tiles[i].blk / tiles[i].tpr;
-      const long long rounds = (d->outer + groups - 1) / groups;
-      return {i, rounds <= (tiles[i].tpr <= 64 ? 4 : 1) ? 1 : even_blocks(rounds, 256)};
+    if (i == TINY) return {TINY, even_blocks((d->outer + TINY_THREADS - 1) / TINY_THREADS, 512)};
+    if (i == LOOPS) {
+      const long long wide = 64 * (d->bf16 ? 8 : 4), cols = (d->n + wide - 1) / wide;
+      const long long s = lmin((d->outer + 2 * DW_WAVES - 1) / (2 * DW_WAVES), (512 + cols - 1) / cols);
+      return {LOOPS, (int)(s < 1 ? 1 : s)};
     }
-    const long long cols = (d->n + 63) / 64, s = lmin((d->outer + 15) / 16, (2048 + cols - 1) / cols);
-    return {LOOPS, (int)(s < 1 ? 1 : lmin(s, 1024))};
+    // 256 blocks: two partials a CU would be more to add than the second block gains.  One block alone writes dw and db
+    // itself; it is worth that for a few rounds of rows (16 x 512: 4.4 us, in two blocks and ln_finish 5.7).
+    const int groups = tiles[i].blk / tiles[i].tpr;
+    const long long rounds = (d->outer + groups - 1) / groups;
+    return {i, rounds <= (tiles[i].tpr <= 64 ? 4 : 1) ? 1 : even_blocks(rounds, 256)};
   }
   const int key = map_bwd(d);
   const long long blocks = map_blocks(d, key);
@@ -932,23 +1126,25 @@ int forward(const RtgLayerNormDesc* d, const void* x, const void* w, const void*
                 mean, rstd);                                                                                                 \
     return rtg_launch_status();                                                                                              \
   }
-#define LN_MAP(LP, W, CPT)                                                                                                   \
-  case map_key(LP, W, CPT):                                                                                                                    \
-    RTG_KLAUNCH((ln_map_fwd<T, LP, W, CPT>), dim3(p.blocks), dim3(map_block(W)), 0, st, s, xt, w, b, yt, mean, rstd); \
+#define LN_MAP_CASE(VEC, ONE, LP, W, CPT)                                                                                    \
+  case map_key(LP, W, CPT, ONE):                                                                                             \
+    RTG_KLAUNCH((ln_map_fwd<VEC, LP, W, CPT>), dim3(p.blocks), dim3(map_block(W)), 0, st, s, xt, w, b, yt, mean, rstd);         \
     return rtg_launch_status();
   if (is_rows(d)) {
     switch (p.tile) {
       LN_ROW(0) LN_ROW(1) LN_ROW(2) LN_ROW(3) LN_ROW(4) LN_ROW(5) LN_ROW(6) LN_ROW(7) LN_ROW(8) LN_ROW(9)
     }
-    RTG_KLAUNCH(ln_row_loop_fwd<T>, dim3(p.blocks), dim3(LOOP_THREADS), 0, st, s, xt, w, b, yt, mean, rstd);
+    if (p.tile == TINY) RTG_KLAUNCH(ln_tiny_fwd<T>, dim3(p.blocks), dim3(TINY_THREADS), 0, st, s, xt, w, b, yt, mean, rstd);
+    else RTG_KLAUNCH(ln_row_loop_fwd<T>, dim3(p.blocks), dim3(LOOP_THREADS), 0, st, s, xt, w, b, yt, mean, rstd);
   } else {
     switch (p.tile) {
       LN_MAP_FWD(LN_MAP)
+      LN_MAP_ONE(LN_MAP1)
     }
     RTG_KLAUNCH(ln_map_loop_fwd<T>, dim3(p.blocks), dim3(LOOP_THREADS), 0, st, s, xt, w, b, yt, mean, rstd);
   }
 #undef LN_ROW
-#undef LN_MAP
+#undef LN_MAP_CASE
   return rtg_launch_status();
 }
 
@@ -969,11 +1165,13 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
                 dt, part, dw, db);                                                                                           \
     break;                                                                                                                   \
   }
-#define LN_MAP(LP, W, CPT)                                                                                                   \
-  case map_key(LP, W, CPT):                                                                                                                    \
-    RTG_KLAUNCH((ln_map_bwd<T, LP, W, CPT>), dim3(p.blocks), dim3(map_block(W)), 0, st, s, gt, xt, mean, rstd, w, dt, part); \
+#define LN_MAP_CASE(VEC, ONE, LP, W, CPT)                                                                                    \
+  case map_key(LP, W, CPT, ONE):                                                                                             \
+    RTG_KLAUNCH((ln_map_bwd<VEC, LP, W, CPT>), dim3(p.blocks), dim3(map_block(W)), 0, st, s, gt, xt, mean, rstd, w, dt, part);  \
     break;
-  if (is_rows(d) && p.tile != LOOPS) {
+  if (p.tile == TINY) {
+    RTG_KLAUNCH(ln_tiny_bwd<T>, dim3(p.blocks), dim3(TINY_THREADS), 0, st, s, gt, xt, mean, rstd, w, dt, part);
+  } else if (is_rows(d) && p.tile != LOOPS) {
     switch (p.tile) {
       LN_ROW(0) LN_ROW(1) LN_ROW(2) LN_ROW(3) LN_ROW(4) LN_ROW(5) LN_ROW(6) LN_ROW(7) LN_ROW(8) LN_ROW(9)
     }
@@ -984,10 +1182,12 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
       if (rc != RTG_OK) return rc;
     }
     if (params)
-      RTG_KLAUNCH(ln_row_loop_dw<T>, dim3((unsigned)((d->n + 63) / 64), p.blocks), dim3(LOOP_THREADS), 0, st, s, gt, xt, mean, rstd, part, p.blocks);
+      RTG_KLAUNCH(ln_row_loop_dw<T>, dim3((unsigned)rtg_ceil_div(d->n, 64 * RtgVec<T>::N), p.blocks), dim3(LOOP_THREADS), 0, st, s, gt, xt, mean,
+                  rstd, part, p.blocks);
   } else if (p.tile != LOOPS) {
     switch (p.tile) {
       LN_MAP_BWD(LN_MAP)
+      LN_MAP_ONE(LN_MAP1)
     }
   } else {
     if (dx) {
@@ -997,12 +1197,13 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
       if (rc != RTG_OK) return rc;
     }
     if (params)
-      RTG_KLAUNCH(ln_map_loop_dw<T>, dim3((unsigned)lmin(d->n, 1 << 20), p.blocks), dim3(LOOP_THREADS), 0, st, s, gt, xt, mean, rstd, part, p.blocks);
+      RTG_KLAUNCH(ln_map_loop_dw<T>, dim3((unsigned)lmin(d->n, 1 << 20), p.blocks), dim3(TINY_THREADS), 0, st, s, gt, xt, mean, rstd, part,
+                  p.blocks);
   }
 #undef LN_ROW
-#undef LN_MAP
+#undef LN_MAP_CASE
   const int rc = rtg_launch_status();
-  if (rc != RTG_OK || !params || (is_rows(d) && p.tile != LOOPS && p.blocks == 1)) return rc;   // (one block: dw, db are written)
+  if (rc != RTG_OK || !params || (is_rows(d) && p.tile >= 0 && p.blocks == 1)) return rc;   // (one block: dw, db are written)
   RTG_KLAUNCH(ln_finish, dim3((unsigned)rtg_ceil_div(d->n, FIN_COLS), 2), dim3(FIN_COLS * FIN_ROWS), 0, st, (const float*)ws, p.blocks,
               d->n, dw, db, s.pbf);
   return rtg_launch_status();

@@ -25,6 +25,7 @@ __device__ __forceinline__ void rtg_pin(float& v) { asm volatile("" : "+v"(v)); 
 // behind rtg_pin of what was summed from it (else the sums move behind hold() and the vector is kept twice).
 template <class T> struct RtgVec;
 template <> struct RtgVec<float> {
+  using T = float;
   static constexpr int N = 4;
   u32x4 r;
   __device__ __forceinline__ void load(const float* p) { r = *reinterpret_cast<const u32x4_a4*>(p); }
@@ -38,6 +39,7 @@ template <> struct RtgVec<float> {
   __device__ __forceinline__ void hold() {}
 };
 template <> struct RtgVec<rtg_bf16> {
+  using T = rtg_bf16;
   static constexpr int N = 8;
   u32x4 r;
   __device__ __forceinline__ void load(const rtg_bf16* p) { r = *reinterpret_cast<const u32x4_a2*>(p); }
@@ -55,6 +57,19 @@ template <> struct RtgVec<rtg_bf16> {
   }
   __device__ __forceinline__ void zero() { r = u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ void hold() { asm volatile("" : "+v"(r)); }
+};
+
+// a single element in the place of a vector: axes shorter than one
+template <class E> struct RtgOne {
+  using T = E;
+  static constexpr int N = 1;
+  E r;
+  __device__ __forceinline__ void load(const E* p) { r = *p; }
+  __device__ __forceinline__ void store(E* p) const { *p = r; }
+  __device__ __forceinline__ float get(int) const { return rtg_up(r); }
+  __device__ __forceinline__ void set(const float (&v)[1]) { rtg_down(v[0], r); }
+  __device__ __forceinline__ void zero() { r = E{}; }
+  __device__ __forceinline__ void hold() {}
 };
 
 // v + (v of another lane), by vector instructions alone (a shuffle goes through LDS: six of them are ~400 cycles of a short
