@@ -257,7 +257,7 @@ def verify(s, norm, want, got):
 
 @pytest.mark.parametrize('off', [0, 1])
 @pytest.mark.parametrize('limit', [0.4, 1e6])
-@pytest.mark.parametrize('sizes', [[1], [3, 5], [4096, 4097, 1023], [300_001, 17], [2_748_371], [50] * 40])
+@pytest.mark.parametrize('sizes', [[1], [3, 5], [4096, 4097, 1023], [300_001, 17], [2_748_371], [50] * 40, [5_000_003, 12_000_001], [1000] * 32])
 def test_update(sizes, limit, off):
     s = state(sizes, 1, off)
     g = [t.clone() for t in s['g']]
