@@ -1348,7 +1348,9 @@ class _NormPlan:
         for size in shape:
             numel *= size
         outer, inner = _axes(shape, stride, 0, dim), _axes(shape, stride, dim + 1, len(shape))
-        self.desc, self.n, self.elements = None, n, numel
+        self.desc, self.n, self.dim, self.bytes = None, n, dim, numel * (2 if bf else 4)
+        # channels that are adjacent in memory are rows, whatever axis they are called
+        self.as_rows = dim != len(shape) - 1 and n > 1 and stride[dim] == 1
         if numel == 0:
             self.desc = L.LayerNormDesc(0, n, 1, 0, 1, bf, pbf, eps)
         elif outer and inner and (inner[0] == 1 and (n == 1 or stride[dim] == 1) or inner[0] > 1 and inner[1] == 1):
@@ -1365,6 +1367,7 @@ class _NormPlan:
 
 
 _norm_plan = functools.lru_cache(maxsize=4096)(_NormPlan)
+_NORM_SEEN = {}           # what a call looks like (shapes, layouts, types, devices, eps, axis) -> its plan, once it has passed the checks
 
 
 def _norm_operands(x, kind, eps, dim):
@@ -1396,21 +1399,40 @@ def _check_norm(x, weight, bias, eps, dim):
     return dim % dims
 
 
+def _looks(t):
+    return None if t is None else (t.shape, t.dtype, t.get_device())
+
+
+def _norm_call(x, weight, bias, eps, dim):
+    """the checks and the plan of a call; calls that look alike are checked once"""
+    here = x.get_device()
+    key = (x.shape, x.stride(), x.dtype, here, _looks(weight), _looks(bias), eps, dim)
+    p = _NORM_SEEN.get(key)
+    if p is None or here != torch._C._cuda_getDevice():
+        d = _check_norm(x, weight, bias, eps, dim)
+        like = weight if weight is not None else bias
+        p = _norm_plan(x.shape, x.stride(), d, x.dtype is _BF, like is not None and like.dtype is _BF, eps)
+        if len(_NORM_SEEN) >= 4096:
+            _NORM_SEEN.clear()
+        _NORM_SEEN[key] = p
+    return p
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _norm_forward(x, weight, bias, eps, dim, keep):
-    """checked operands -> (y, statistics [mean | rstd] or None, x as read, the plan)"""
+def _norm_forward(x, weight, bias, eps, p, keep):
+    """checked operands and their plan -> (y, statistics [mean | rstd] or None, x as read, the plan it was read with)"""
+    if p.desc is None:
+        like = weight if weight is not None else bias
+        x, p = _norm_operands(x, None if like is None else like.dtype, eps, p.dim)
     weight, bias = _c(weight), _c(bias)
-    like = weight if weight is not None else bias
-    x, p = _norm_operands(x, None if like is None else like.dtype, eps, dim)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     stats = torch.empty(2 * p.rows, device=x.device) if keep else None
     mean = stats.data_ptr() if keep else None
-    rstd = mean + 4 * p.rows if keep else None
-    st = timed_bw('layernorm_fwd', 2 * x.element_size() * p.elements, lambda: lib.rtg_layernorm_forward(
-        p.ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean, rstd, _stream()))
+    args = (p.ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean, mean + 4 * p.rows if keep else None, _stream())
+    st = lib.rtg_layernorm_forward(*args) if PROFILE is None else timed_bw('layernorm_fwd', 2 * p.bytes, lambda: lib.rtg_layernorm_forward(*args))
     if st:
         check(st, 'layernorm forward')
     return y, stats, x, p
@@ -1424,8 +1446,8 @@ def _norm_backward(dy, x, mean, rstd, weight, p, kind, needs):
     dw = torch.empty(p.n, device=dev, dtype=kind) if needs[1] else None
     db = torch.empty(p.n, device=dev, dtype=kind) if needs[2] else None
     ws = torch.empty(p.scratch(), device=dev) if needs[1] or needs[2] else None
-    st = timed_bw('layernorm_bwd', 3 * x.element_size() * p.elements, lambda: lib.rtg_layernorm_backward(
-        p.ref, dy.data_ptr(), x.data_ptr(), mean, rstd, _ptr(weight), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), _stream()))
+    args = (p.ref, dy.data_ptr(), x.data_ptr(), mean, rstd, _ptr(weight), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), _stream())
+    st = lib.rtg_layernorm_backward(*args) if PROFILE is None else timed_bw('layernorm_bwd', 3 * p.bytes, lambda: lib.rtg_layernorm_backward(*args))
     if st:
         check(st, 'layernorm backward')
     return dx, dw, db
@@ -1434,7 +1456,7 @@ def _norm_backward(dy, x, mean, rstd, weight, p, kind, needs):
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, dim=-1, keep=False):
     """layer_norm without autograd -> y, or with `keep` (y, mean, rstd): the statistics (float32, one per row or position)
     that layer_norm_backward reads"""
-    y, stats, _, p = _norm_forward(x, weight, bias, eps, _check_norm(x, weight, bias, eps, dim), keep)
+    y, stats, _, p = _norm_forward(x, weight, bias, eps, _norm_call(x, weight, bias, eps, dim), keep)
     return (y, stats[:p.rows], stats[p.rows:]) if keep else y
 
 
@@ -1456,8 +1478,8 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, dim=-1, needs=(True, Tru
 
 class LayerNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, dim):
-        y, stats, x, ctx.plan = _norm_forward(x, weight, bias, eps, dim, True)
+    def forward(ctx, x, weight, bias, eps, plan):
+        y, stats, x, ctx.plan = _norm_forward(x, weight, bias, eps, plan, True)
         ctx.save_for_backward(x, weight, stats)
         ctx.kind = weight.dtype if weight is not None else (torch.float32 if bias is None else bias.dtype)
         return y
@@ -1481,13 +1503,13 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
     float32 or bfloat16 of shape (n,), or None.  Strided rows, time crops and channel slices of a map are read in place, and a
     map whose channels are adjacent ([B, T, C] transposed) takes the row kernels; the result is as dense as x is.  One launch
     forward, two backward (gradients of x, weight and bias, summed in a fixed order); not differentiable twice."""
-    d = _check_norm(x, weight, bias, eps, dim)
-    if d != x.dim() - 1 and x.stride(d) == 1 and x.shape[d] > 1:          # the channels are adjacent: rows
-        return layer_norm(x.movedim(d, -1), weight, bias, eps, -1).movedim(-1, d)
+    p = _norm_call(x, weight, bias, eps, dim)
+    if p.as_rows:
+        return layer_norm(x.movedim(p.dim, -1), weight, bias, eps, -1).movedim(-1, p.dim)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
-        return LayerNormFn.apply(x, weight, bias, eps, d)
-    return _norm_forward(x, weight, bias, eps, d, False)[0]
+        return LayerNormFn.apply(x, weight, bias, eps, p)
+    return _norm_forward(x, weight, bias, eps, p, False)[0]
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -1534,7 +1556,8 @@ class _GradList:
         if not found.issubset(_NORM_TYPES):
             i = next(i for i, k in enumerate(kinds) if k not in _NORM_TYPES)
             raise L.RtgError(f'{what}: gradient {i} is {kinds[i]} (float32 or bfloat16)')
-        if set(map(_TB.get_device, ts)) != {torch.cuda.current_device() if torch.cuda.is_available() else None}:
+        places = set(map(_TB.get_device, ts))
+        if len(places) > 1 or -1 in places or places != {torch.cuda.current_device()}:
             _need_here(what, *ts)
         n = len(ts)
         try:
