@@ -30,6 +30,12 @@ template <> struct RtgVec<float> {
   u32x4 r;
   __device__ __forceinline__ void load(const float* p) { r = *reinterpret_cast<const u32x4_a4*>(p); }
   __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<u32x4_a4*>(p) = r; }
+  // ... that nobody reads again soon: the line leaves the caches first
+  __device__ __forceinline__ void load_once(const float* p) { r = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a4*>(p)); }
+  __device__ __forceinline__ void store_once(float* p) const {
+    const u32x4_a4 v = r;
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_a4*>(p));
+  }
   __device__ __forceinline__ float get(int e) const { return __uint_as_float(r[e]); }
   __device__ __forceinline__ void set(const float (&v)[4]) {
 #pragma unroll
