@@ -97,7 +97,7 @@ __device__ __forceinline__ int odd_head(const T* p, long long n) {
   return sizeof(T) == 2 && n > 0 && (reinterpret_cast<uintptr_t>(p) & 2) ? 1 : 0;
 }
 
-template <class T, int KIND>
+template <class T, int KIND, bool ONCE>
 __device__ __forceinline__ double chunk_sum(const T* __restrict__ p, long long n) {
   constexpr int N = RtgVec<T>::N;
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
@@ -110,7 +110,7 @@ __device__ __forceinline__ double chunk_sum(const T* __restrict__ p, long long n
   for (; i + 3 * THREADS < nv; i += 4 * THREADS) {
     RtgVec<T> v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k].load(p + (i + k * THREADS) * N);
+    for (int k = 0; k < 4; ++k) rtg_load<ONCE>(v[k], p + (i + k * THREADS) * N);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -118,7 +118,7 @@ __device__ __forceinline__ double chunk_sum(const T* __restrict__ p, long long n
   }
   for (; i < nv; i += THREADS) {
     RtgVec<T> v;
-    v.load(p + i * N);
+    rtg_load<ONCE>(v, p + i * N);
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[0] = take<KIND>(acc[0], v.get(e));
   }
@@ -139,25 +139,33 @@ __device__ __forceinline__ Piece piece_of(const GradTable& t) {
   return r;
 }
 
-template <int KIND>
+// Who reads a tensor again, and from where: a list of up to CACHED bytes is still in the memory-side cache (256 MB) when the
+// scaling or the update comes, so its norm leaves it there and the scaling, its last reader, makes no room for what it reads and
+// writes (27 M floats clipped 69.5 -> 62.0 us; with both passes that way 74, the second then reads HBM).  Of a longer list
+// nothing is left by then: its norm reads past the caches (1 GB of bf16 204 -> 187 us, 5.75 TB/s; clipped 678 -> 623).
+constexpr long long CACHED = 256ll << 20;
+
+template <int KIND, bool ONCE>
 __global__ __launch_bounds__(THREADS) void grad_partial(const GradTable t, double* __restrict__ part) {
   __shared__ double red[THREADS / 64];
   const Piece c = piece_of(t);
   double acc;
-  if (c.bf) acc = chunk_sum<rtg_bf16, KIND>(reinterpret_cast<const rtg_bf16*>(t.p[c.i]) + c.lo, c.n);
-  else acc = chunk_sum<float, KIND>(reinterpret_cast<const float*>(t.p[c.i]) + c.lo, c.n);
+  if (c.bf) acc = chunk_sum<rtg_bf16, KIND, ONCE>(reinterpret_cast<const rtg_bf16*>(t.p[c.i]) + c.lo, c.n);
+  else acc = chunk_sum<float, KIND, ONCE>(reinterpret_cast<const float*>(t.p[c.i]) + c.lo, c.n);
   acc = block_join<KIND, THREADS>(acc, red);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
 
 template <int KIND>
-__global__ __launch_bounds__(REDUCE) void grad_norm_finish(const double* __restrict__ part, int n, float* __restrict__ out) {
+__global__ __launch_bounds__(REDUCE) void grad_norm_finish(double* part, int n, float* __restrict__ out, int joined) {
   __shared__ double red[REDUCE / 64];
-  const double norm = norm_of<KIND>(all_partials<KIND, REDUCE>(part, n, red));
-  if (threadIdx.x == 0) *out = (float)norm;
+  const double acc = all_partials<KIND, REDUCE>(part, n, red);
+  if (threadIdx.x != 0) return;
+  *out = (float)norm_of<KIND>(acc);
+  if (joined) part[0] = acc;                             // (behind the barriers of the sum: all have read it)
 }
 
-template <class T>
+template <class T, bool ONCE>
 __device__ __forceinline__ void chunk_scale(T* __restrict__ p, long long n, float f) {
   constexpr int N = RtgVec<T>::N;
   const int head = odd_head(p, n);
@@ -168,18 +176,20 @@ __device__ __forceinline__ void chunk_scale(T* __restrict__ p, long long n, floa
   for (long long i = threadIdx.x; i < nv; i += THREADS) {
     RtgVec<T> v;
     float r[N];
-    v.load(p + i * N);
+    rtg_load<ONCE>(v, p + i * N);
 #pragma unroll
     for (int e = 0; e < N; ++e) r[e] = v.get(e) * f;
     v.set(r);
-    v.store(p + i * N);
+    rtg_store<ONCE>(v, p + i * N);
   }
   if (nv * N + threadIdx.x < n) rtg_down(rtg_up(p[nv * N + threadIdx.x]) * f, p[nv * N + threadIdx.x]);
 }
 
-// every workgroup joins the partials by itself (they sit in L2; a launch of one workgroup for it costs more) and scales the
-// chunk whose sum it may have taken
-template <int KIND>
+// scales the chunk whose sum it may have taken.  Up to JOIN_FIRST partials every workgroup joins them by itself (they sit in L2;
+// a launch of one workgroup for it costs more: 2.7 M elements 13.1 us, with it 14.7); of more, the first one holds what that
+// launch made of them (2 GB of floats within the limit 459 -> 426 us, 30000 tensors 1931 -> 1386)
+constexpr int JOIN_FIRST = 4096;
+template <int KIND, bool ONCE>
 __global__ __launch_bounds__(THREADS) void grad_scale(const GradTable t, const double* __restrict__ part, int n_part, double max_norm,
                                                       float* __restrict__ out, int write_norm) {
   __shared__ double red[THREADS / 64];
@@ -188,8 +198,8 @@ __global__ __launch_bounds__(THREADS) void grad_scale(const GradTable t, const d
   const float f = clip_factor(norm, max_norm);
   if (f == 1.f) return;
   const Piece c = piece_of(t);
-  if (c.bf) chunk_scale(reinterpret_cast<rtg_bf16*>(t.p[c.i]) + c.lo, c.n, f);
-  else chunk_scale(reinterpret_cast<float*>(t.p[c.i]) + c.lo, c.n, f);
+  if (c.bf) chunk_scale<rtg_bf16, ONCE>(reinterpret_cast<rtg_bf16*>(t.p[c.i]) + c.lo, c.n, f);
+  else chunk_scale<float, ONCE>(reinterpret_cast<float*>(t.p[c.i]) + c.lo, c.n, f);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -240,7 +250,7 @@ __global__ __launch_bounds__(THREADS) void adam_partial(const AdamTable t, doubl
   const int j = entry_of(t.first, t.count, blockIdx.x);
   const long long lo = (long long)((int)blockIdx.x - t.first[j]) * t.chunk;
   const long long left = t.job[j].n - lo;
-  const double sum = block_join<RTG_NORM_L2, THREADS>(chunk_sum<float, RTG_NORM_L2>(t.job[j].grads + lo, left < t.chunk ? left : t.chunk), red);
+  const double sum = block_join<RTG_NORM_L2, THREADS>(chunk_sum<float, RTG_NORM_L2, false>(t.job[j].grads + lo, left < t.chunk ? left : t.chunk), red);
   if (threadIdx.x != 0) return;
   part[blockIdx.x] = sum;
   if ((int)blockIdx.x == t.first[j]) held[j] = AdamScalars{t.job[j].step_state[0], 0.f, 0.f, adam_flagged(t.job[j].loss_flag) ? 0.f : 1.f};
@@ -282,17 +292,10 @@ __global__ __launch_bounds__(THREADS) void adam_update(const AdamTable t, const 
   const long long nv = n / 4;
   for (long long i = threadIdx.x; i < nv; i += THREADS) {
     RtgVec<float> a, b, c, d;
-    if constexpr (FEW) {
-      a.load(p + 4 * i);
-      b.load(g + 4 * i);
-      c.load(m + 4 * i);
-      d.load(v + 4 * i);
-    } else {
-      a.load_once(p + 4 * i);
-      b.load_once(g + 4 * i);
-      c.load_once(m + 4 * i);
-      d.load_once(v + 4 * i);
-    }
+    rtg_load<!FEW>(a, p + 4 * i);
+    rtg_load<!FEW>(b, g + 4 * i);
+    rtg_load<!FEW>(c, m + 4 * i);
+    rtg_load<!FEW>(d, v + 4 * i);
     float pr[4], mr[4], vr[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -304,15 +307,9 @@ __global__ __launch_bounds__(THREADS) void adam_update(const AdamTable t, const 
     a.set(pr);
     c.set(mr);
     d.set(vr);
-    if constexpr (FEW) {
-      a.store(p + 4 * i);
-      c.store(m + 4 * i);
-      d.store(v + 4 * i);
-    } else {
-      a.store_once(p + 4 * i);
-      c.store_once(m + 4 * i);
-      d.store_once(v + 4 * i);
-    }
+    rtg_store<!FEW>(a, p + 4 * i);
+    rtg_store<!FEW>(c, m + 4 * i);
+    rtg_store<!FEW>(d, v + 4 * i);
   }
   const long long i = 4 * nv + threadIdx.x;
   if (i < n) step(p[i], g[i], m[i], v[i]);
@@ -333,11 +330,15 @@ long long chunk_bytes(long long total) {
   return c > least ? c : least;
 }
 
-// walks the list, TABLE tensors a launch: launch(table, workgroups, workgroups before) for each -> status; *blocks: all of them
-template <class F>
-int each_table(int n, void* const* grads, const long long* counts, const int* bf16, int* blocks, F launch) {
+long long list_bytes(int n, const long long* counts, const int* bf16) {
   long long total = 0;
   for (int i = 0; i < n; ++i) total += counts[i] * (bf16[i] ? 2 : 4);
+  return total;
+}
+
+// walks the list, TABLE tensors a launch: launch(table, workgroups, workgroups before) for each -> status; *blocks: all of them
+template <class F>
+int each_table(int n, void* const* grads, const long long* counts, const int* bf16, long long total, int* blocks, F launch) {
   GradTable t;
   t.chunk = chunk_bytes(total);
   int before = 0, here = 0;
@@ -392,9 +393,10 @@ int disjoint(Range* r, long long n) {
 }
 
 template <int KIND>
-int partials(int n, void* const* grads, const long long* counts, const int* bf16, double* ws, int* blocks, hipStream_t st) {
-  return each_table(n, grads, counts, bf16, blocks, [&](const GradTable& t, int here, int before) {
-    RTG_KLAUNCH(grad_partial<KIND>, dim3(here), dim3(THREADS), 0, st, t, ws + before);
+int partials(int n, void* const* grads, const long long* counts, const int* bf16, long long total, double* ws, int* blocks, hipStream_t st) {
+  return each_table(n, grads, counts, bf16, total, blocks, [&](const GradTable& t, int here, int before) {
+    if (total > CACHED) RTG_KLAUNCH((grad_partial<KIND, true>), dim3(here), dim3(THREADS), 0, st, t, ws + before);
+    else RTG_KLAUNCH((grad_partial<KIND, false>), dim3(here), dim3(THREADS), 0, st, t, ws + before);
     return rtg_launch_status();
   });
 }
@@ -402,23 +404,30 @@ int partials(int n, void* const* grads, const long long* counts, const int* bf16
 template <int KIND>
 int norm(int n, void* const* grads, const long long* counts, const int* bf16, double* ws, float* out, hipStream_t st) {
   int blocks = 0;
-  const int rc = partials<KIND>(n, grads, counts, bf16, ws, &blocks, st);
+  const int rc = partials<KIND>(n, grads, counts, bf16, list_bytes(n, counts, bf16), ws, &blocks, st);
   if (rc != RTG_OK) return rc;
-  RTG_KLAUNCH(grad_norm_finish<KIND>, dim3(1), dim3(REDUCE), 0, st, (const double*)ws, blocks, out);
+  RTG_KLAUNCH(grad_norm_finish<KIND>, dim3(1), dim3(REDUCE), 0, st, ws, blocks, out, 0);
   return rtg_launch_status();
 }
 
 template <int KIND>
 int clip(int n, void* const* grads, const long long* counts, const int* bf16, double max_norm, double* ws, float* out, hipStream_t st) {
+  const long long total = list_bytes(n, counts, bf16);
   int blocks = 0, again = 0;
-  const int rc = partials<KIND>(n, grads, counts, bf16, ws, &blocks, st);
+  const int rc = partials<KIND>(n, grads, counts, bf16, total, ws, &blocks, st);
   if (rc != RTG_OK) return rc;
-  if (blocks == 0) {                                     // nothing but empty tensors: the norm is 0
-    RTG_KLAUNCH(grad_norm_finish<KIND>, dim3(1), dim3(REDUCE), 0, st, (const double*)ws, 0, out);
-    return rtg_launch_status();
+  const bool first = blocks == 0 || blocks > JOIN_FIRST;      // (nothing but empty tensors: the norm is 0)
+  if (first) {
+    RTG_KLAUNCH(grad_norm_finish<KIND>, dim3(1), dim3(REDUCE), 0, st, ws, blocks, out, (int)(blocks > 0));
+    const int joined = rtg_launch_status();
+    if (joined != RTG_OK || blocks == 0) return joined;
   }
-  return each_table(n, grads, counts, bf16, &again, [&](const GradTable& t, int here, int before) {
-    RTG_KLAUNCH(grad_scale<KIND>, dim3(here), dim3(THREADS), 0, st, t, (const double*)ws, blocks, max_norm, out, (int)(before == 0));
+  return each_table(n, grads, counts, bf16, total, &again, [&](const GradTable& t, int here, int before) {
+    const int parts = first ? 1 : blocks, write_norm = before == 0 && !first;
+    if (total > CACHED)
+      RTG_KLAUNCH((grad_scale<KIND, false>), dim3(here), dim3(THREADS), 0, st, t, (const double*)ws, parts, max_norm, out, write_norm);
+    else
+      RTG_KLAUNCH((grad_scale<KIND, true>), dim3(here), dim3(THREADS), 0, st, t, (const double*)ws, parts, max_norm, out, write_norm);
     return rtg_launch_status();
   });
 }
@@ -476,7 +485,7 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
          reinterpret_cast<uintptr_t>(j.exp_avg_sq) | reinterpret_cast<uintptr_t>(j.step_state)) & 3) return RTG_EINVAL;
   }
   {
-    std::unique_ptr<Range[]> r(new (std::nothrow) Range[5 * (size_t)n]);
+    std::unique_ptr<Range[]> r(new (std::nothrow) Range[5 * (size_t)n + 1]);
     if (!r) return RTG_ERANGE;
     for (int i = 0; i < n; ++i) {
       const RtgAdamWJob& j = jobs[i];
@@ -486,7 +495,9 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
         r[5 * (size_t)i + k] = Range{lo, lo + (k < 4 ? 4 * (uintptr_t)j.n : 4)};
       }
     }
-    const int apart = disjoint(r.get(), 5ll * n);
+    const uintptr_t out = reinterpret_cast<uintptr_t>(norm_out);
+    r[5 * (size_t)n] = Range{out, out + (out ? 4 : 0)};
+    const int apart = disjoint(r.get(), 5ll * n + 1);
     if (apart != RTG_OK) return apart;
   }
   hipStream_t st = (hipStream_t)stream;
@@ -532,7 +543,8 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
       t.first[t.count] = here;
       here += (int)((4 * j.n + t.chunk - 1) / t.chunk);
     }
-    RTG_KLAUNCH(grad_partial<RTG_NORM_L2>, dim3(here), dim3(THREADS), 0, st, t, ws + blocks);
+    if (4 * total > CACHED) RTG_KLAUNCH((grad_partial<RTG_NORM_L2, true>), dim3(here), dim3(THREADS), 0, st, t, ws + blocks);
+    else RTG_KLAUNCH((grad_partial<RTG_NORM_L2, false>), dim3(here), dim3(THREADS), 0, st, t, ws + blocks);
     const int rc = rtg_launch_status();
     if (rc != RTG_OK) return rc;
     blocks += here;

@@ -30,7 +30,7 @@ template <> struct RtgVec<float> {
   u32x4 r;
   __device__ __forceinline__ void load(const float* p) { r = *reinterpret_cast<const u32x4_a4*>(p); }
   __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<u32x4_a4*>(p) = r; }
-  // ... that nobody reads again soon: the line leaves the caches first
+  // ... that nobody reads again soon: the line is the first to leave the caches
   __device__ __forceinline__ void load_once(const float* p) { r = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a4*>(p)); }
   __device__ __forceinline__ void store_once(float* p) const {
     const u32x4_a4 v = r;
@@ -50,6 +50,11 @@ template <> struct RtgVec<rtg_bf16> {
   u32x4 r;
   __device__ __forceinline__ void load(const rtg_bf16* p) { r = *reinterpret_cast<const u32x4_a2*>(p); }
   __device__ __forceinline__ void store(rtg_bf16* p) const { *reinterpret_cast<u32x4_a2*>(p) = r; }
+  __device__ __forceinline__ void load_once(const rtg_bf16* p) { r = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a2*>(p)); }
+  __device__ __forceinline__ void store_once(rtg_bf16* p) const {
+    const u32x4_a2 v = r;
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_a2*>(p));
+  }
   __device__ __forceinline__ float get(int e) const {
     return __uint_as_float(e & 1 ? r[e >> 1] & 0xffff0000u : r[e >> 1] << 16);
   }
@@ -64,6 +69,17 @@ template <> struct RtgVec<rtg_bf16> {
   __device__ __forceinline__ void zero() { r = u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ void hold() { asm volatile("" : "+v"(r)); }
 };
+
+template <bool ONCE, class V, class T>
+__device__ __forceinline__ void rtg_load(V& v, const T* p) {
+  if constexpr (ONCE) v.load_once(p);
+  else v.load(p);
+}
+template <bool ONCE, class V, class T>
+__device__ __forceinline__ void rtg_store(const V& v, T* p) {
+  if constexpr (ONCE) v.store_once(p);
+  else v.store(p);
+}
 
 // a single element in the place of a vector: axes shorter than one
 template <class E> struct RtgOne {
