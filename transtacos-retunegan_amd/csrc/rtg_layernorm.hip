@@ -16,8 +16,13 @@ struct LnShape {
   long long outer, n, inner, xo, xn;      // x[o * xo + c * xn + t]; everything else contiguous
   float nf, inv_n, eps;                   // n, 1 / n
   int pbf;                                // weight / bias (and their gradients) are bf16
+  int once;                               // what is read goes by the caches: below
 };
 
+// What a kernel reads goes by the caches where that much is not in the memory-side cache (256 MB) when somebody reads it next:
+// 16384 x 4096 floats 95 -> 83 us forward, 154 -> 129 backward, (32, 128, 16384) floats 109 -> 83 and 171 -> 144; of 64 MB it
+// costs up to a tenth, a neighbour's part of a shared line comes twice then.
+constexpr long long CACHED = 256ll << 20;
 // sum / n: one multiplication and its correction by the remainder (what a division comes to, without its range checks: n is a
 // plain number), so that the mean of equal values is that value
 __device__ __forceinline__ float mean_of(float sum, const LnShape& s) {
@@ -124,7 +129,7 @@ struct RowLane {
 };
 
 // AHEAD 0 (rows of 1024 threads, 128 registers each): neither the weights nor the next row are held
-template <class T, int TPR, int VPT, int BLK, int AHEAD>
+template <class T, int TPR, int VPT, int BLK, int AHEAD, bool ONCE>
 __global__ __launch_bounds__(BLK) void ln_row_fwd(LnShape s, const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b,
                                                   T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   constexpr int N = RtgVec<T>::N, G = BLK / TPR;
@@ -138,7 +143,7 @@ __global__ __launch_bounds__(BLK) void ln_row_fwd(LnShape s, const T* __restrict
   RtgVec<T> v[VPT], next[VPT];
   float wr[AHEAD ? VPT : 1][N], br[AHEAD ? VPT : 1][N];
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) next[k].load(x + row * s.xo + at.col[k]);
+  for (int k = 0; k < VPT; ++k) rtg_load<ONCE>(next[k], x + row * s.xo + at.col[k]);
   if constexpr (AHEAD) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(BLK) void ln_row_fwd(LnShape s, const T* __restrict
     const T* xn = x + (row + step < s.outer ? row + step : row) * s.xo;
     if constexpr (AHEAD) {
 #pragma unroll
-      for (int k = 0; k < VPT; ++k) next[k].load(xn + at.col[k]);
+      for (int k = 0; k < VPT; ++k) rtg_load<ONCE>(next[k], xn + at.col[k]);
     }
     float a[1] = {0.f};
 #pragma unroll
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(BLK) void ln_row_fwd(LnShape s, const T* __restrict
     }
     if constexpr (!AHEAD) {
 #pragma unroll
-      for (int k = 0; k < VPT; ++k) next[k].load(xn + at.col[k]);
+      for (int k = 0; k < VPT; ++k) rtg_load<ONCE>(next[k], xn + at.col[k]);
     }
     if (mean_out && t == 0) {
       mean_out[row] = mean;
@@ -203,7 +208,7 @@ __global__ __launch_bounds__(BLK) void ln_row_fwd(LnShape s, const T* __restrict
 
 // dx, and the block's share of dw and db: a thread owns the same columns of every row its block walks, so their sums stay in
 // registers; the groups of a block add theirs in LDS at the end, and ln_finish adds the blocks'.
-template <class T, int TPR, int VPT, int BLK, int AHEAD>
+template <class T, int TPR, int VPT, int BLK, int AHEAD, bool ONCE>
 __global__ __launch_bounds__(BLK) void ln_row_bwd(LnShape s, const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean_in,
                                                   const float* __restrict__ rstd_in, const void* __restrict__ w, T* __restrict__ dx,
                                                   float* __restrict__ part, void* __restrict__ dw, void* __restrict__ db) {
@@ -219,8 +224,8 @@ __global__ __launch_bounds__(BLK) void ln_row_bwd(LnShape s, const T* __restrict
     row = row < last ? row : last;                         // (a group behind the last row works on it once more, for nothing)
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      xd[k].load(x + row * s.xo + at.col[k]);
-      gd[k].load(dy + row * s.n + at.col[k]);
+      rtg_load<ONCE>(xd[k], x + row * s.xo + at.col[k]);
+      rtg_load<ONCE>(gd[k], dy + row * s.n + at.col[k]);
     }
     m = mean_in[row];
     r = rstd_in[row];
@@ -389,14 +394,27 @@ struct MapLane {
   __device__ __forceinline__ static const T* byte(const T* p, unsigned off) {
     return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + off);
   }
-  __device__ __forceinline__ void load(V (&v)[CPT], const T* p, long long outer, long long stride) const {
-    p += o * outer;
-    if (full) {
+  // f(i) -> where vector i lies.  The fences keep the branches apart (merged, the loads would be of the plain kind); a loop that
+  // has the next loads in flight cannot take such a branch, so the row kernels are built both ways
+  __device__ __forceinline__ static void fence() { asm volatile("" ::: "memory"); }
+  template <class F>
+  __device__ __forceinline__ static void fetch(V (&v)[CPT], int once, F f) {
+    if (once) {
+      fence();
 #pragma unroll
-      for (int i = 0; i < CPT; ++i) v[i].load(byte(p + (cw + i * M::CL * W) * stride, off(stride)));
+      for (int i = 0; i < CPT; ++i) v[i].load_once(f(i));
+      fence();
     } else {
 #pragma unroll
-      for (int i = 0; i < CPT; ++i) v[i].load(byte(p + base(i) * stride, has(i) ? off(stride) : off0()));
+      for (int i = 0; i < CPT; ++i) v[i].load(f(i));
+    }
+  }
+  __device__ __forceinline__ void load(V (&v)[CPT], const T* p, long long outer, long long stride, int once) const {
+    p += o * outer;
+    if (full) {
+      fetch(v, once, [&](int i) __attribute__((always_inline)) { return byte(p + (cw + i * M::CL * W) * stride, off(stride)); });
+    } else {
+      fetch(v, once, [&](int i) __attribute__((always_inline)) { return byte(p + base(i) * stride, has(i) ? off(stride) : off0()); });
 #pragma unroll
       for (int i = 0; i < CPT; ++i)
         if (!has(i)) v[i].zero();
@@ -442,7 +460,7 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_fwd(LnShape s, const T* _
   const unsigned per = (unsigned)((s.inner + M::POS - 1) / M::POS);
   at.go(s, xcd_order(blockIdx.x, gridDim.x) * M::TEAMS + at.wave / W, (unsigned)s.outer * per, per);
   V v[CPT];
-  at.load(v, x, s.xo, s.xn);
+  at.load(v, x, s.xo, s.xn, s.once);
   float wr[CPT], br[CPT], a[N], mean[N], rstd[N];
   at.params(wr, w, s.pbf, 1.f);
   at.params(br, b, s.pbf, 0.f);
@@ -511,8 +529,8 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* _
   for (unsigned base = xcd_order(blockIdx.x, gridDim.x) * M::TEAMS; base < tiles; base += gridDim.x * M::TEAMS, turn ^= 1) {
     at.go(s, base + team, tiles, per);
     V xv[CPT], gv[CPT];
-    at.load(xv, x, s.xo, s.xn);
-    at.load(gv, dy, s.n * s.inner, s.inner);
+    at.load(xv, x, s.xo, s.xn, s.once);
+    at.load(gv, dy, s.n * s.inner, s.inner, s.once);
     float mean[N], rstd[N], a[2 * N];
     load_params<N>(mean, mean_in, 0, at.o * s.inner + at.t, 0.f);
     load_params<N>(rstd, rstd_in, 0, at.o * s.inner + at.t, 0.f);
@@ -962,8 +980,10 @@ int check_desc(const RtgLayerNormDesc* d) {
   return RTG_OK;
 }
 
-LnShape shape_of(const RtgLayerNormDesc* d) {
-  return LnShape{d->outer, d->n, d->inner, d->x_outer, d->x_n, (float)d->n, (float)(1.0 / (double)d->n), d->eps, d->param_bf16 != 0};
+// tensors: how many of the problem's size a kernel reads
+LnShape shape_of(const RtgLayerNormDesc* d, int tensors) {
+  return LnShape{d->outer, d->n, d->inner, d->x_outer, d->x_n, (float)d->n, (float)(1.0 / (double)d->n), d->eps, d->param_bf16 != 0,
+                 d->outer * d->n * d->inner >= CACHED / ((d->bf16 ? 2 : 4) * tensors)};
 }
 
 bool is_rows(const RtgLayerNormDesc* d) { return d->inner == 1; }
@@ -1115,15 +1135,18 @@ Plan plan_bwd(const RtgLayerNormDesc* d) {
 
 template <class T>
 int forward(const RtgLayerNormDesc* d, const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, hipStream_t st) {
-  const LnShape s = shape_of(d);
+  const LnShape s = shape_of(d, 1);
   const T* xt = reinterpret_cast<const T*>(x);
   T* yt = reinterpret_cast<T*>(y);
   const Plan p = plan_fwd(d);
 #define LN_ROW(I)                                                                                                            \
   case I: {                                                                                                                  \
     constexpr RowTile R = FWD_TILES[I];                                                                                      \
-    RTG_KLAUNCH((ln_row_fwd<T, R.tpr, R.vpt, R.blk, (R.tpr * R.vpt < 4096)>), dim3(p.blocks), dim3(R.blk), 0, st, s, xt, w, b, yt, \
-                mean, rstd);                                                                                                 \
+    constexpr int AHEAD = R.tpr * R.vpt < 4096;                                                                              \
+    if (s.once)                                                                                                              \
+      RTG_KLAUNCH((ln_row_fwd<T, R.tpr, R.vpt, R.blk, AHEAD, true>), dim3(p.blocks), dim3(R.blk), 0, st, s, xt, w, b, yt, mean, rstd); \
+    else                                                                                                                     \
+      RTG_KLAUNCH((ln_row_fwd<T, R.tpr, R.vpt, R.blk, AHEAD, false>), dim3(p.blocks), dim3(R.blk), 0, st, s, xt, w, b, yt, mean, rstd); \
     return rtg_launch_status();                                                                                              \
   }
 #define LN_MAP_CASE(VEC, ONE, LP, W, CPT)                                                                                    \
@@ -1151,7 +1174,7 @@ int forward(const RtgLayerNormDesc* d, const void* x, const void* w, const void*
 template <class T>
 int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const float* mean, const float* rstd, const void* w, void* dx,
              void* dw, void* db, float* ws, hipStream_t st) {
-  const LnShape s = shape_of(d);
+  const LnShape s = shape_of(d, 2);
   const T *xt = reinterpret_cast<const T*>(x), *gt = reinterpret_cast<const T*>(dy);
   T* dt = reinterpret_cast<T*>(dx);
   const bool params = dw || db;
@@ -1161,8 +1184,13 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
 #define LN_ROW(I)                                                                                                            \
   case I: {                                                                                                                  \
     constexpr RowTile R = sizeof(T) == 2 ? BWD_BF16[I] : BWD_F32[I];                                                         \
-    RTG_KLAUNCH((ln_row_bwd<T, R.tpr, R.vpt, R.blk, (R.tpr < 1024)>), dim3(p.blocks), dim3(R.blk), 0, st, s, gt, xt, mean, rstd, w, \
-                dt, part, dw, db);                                                                                           \
+    constexpr int AHEAD = R.tpr < 1024;                                                                                      \
+    if (s.once)                                                                                                              \
+      RTG_KLAUNCH((ln_row_bwd<T, R.tpr, R.vpt, R.blk, AHEAD, true>), dim3(p.blocks), dim3(R.blk), 0, st, s, gt, xt, mean, rstd, w, dt, \
+                  part, dw, db);                                                                                             \
+    else                                                                                                                     \
+      RTG_KLAUNCH((ln_row_bwd<T, R.tpr, R.vpt, R.blk, AHEAD, false>), dim3(p.blocks), dim3(R.blk), 0, st, s, gt, xt, mean, rstd, w, dt, \
+                  part, dw, db);                                                                                             \
     break;                                                                                                                   \
   }
 #define LN_MAP_CASE(VEC, ONE, LP, W, CPT)                                                                                    \

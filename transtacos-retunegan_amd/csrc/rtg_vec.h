@@ -87,6 +87,7 @@ template <class E> struct RtgOne {
   static constexpr int N = 1;
   E r;
   __device__ __forceinline__ void load(const E* p) { r = *p; }
+  __device__ __forceinline__ void load_once(const E* p) { r = *p; }
   __device__ __forceinline__ void store(E* p) const { *p = r; }
   __device__ __forceinline__ float get(int) const { return rtg_up(r); }
   __device__ __forceinline__ void set(const float (&v)[1]) { rtg_down(v[0], r); }
