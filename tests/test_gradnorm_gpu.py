@@ -172,6 +172,36 @@ def test_more_elements_than_32_bits_count():
     assert (t[0].item(), t[n // 2].item(), t[-1].item()) == (1.5, 2.0, 6.0) and t.count_nonzero().item() == 3
 
 
+@pytest.mark.parametrize('kind', [F32, BF])
+@pytest.mark.parametrize('norm_type', [2, float('inf')])
+def test_lists_that_no_cache_holds(norm_type, kind):
+    """more than 256 MB, which are read past the caches, with more partials than a workgroup of the scaling reads by itself"""
+    from rtg import ops
+    flat = torch.randn(150_000_001, generator=torch.Generator(device=DEV).manual_seed(7), device=DEV).to(kind)
+    ts = [t for t in flat[1:].split(31_013)]
+    assert len(ts) > 4096
+    before, norm = flat.clone(), norm64([flat[1:]], norm_type)
+    close(ops.total_norm(ts, norm_type), norm)
+    close(ops.clip_grads_(ts, 2 * norm, norm_type), norm)
+    assert torch.equal(flat, before)
+    close(ops.clip_grads_(ts, 0.3 * norm, norm_type), norm)
+    want = before[1:].double() * (0.3 * norm / (norm + 1e-6))
+    inside(flat[1:], want, (2 * U + half_step(kind) + 1e-9) * want.abs() + 1e-40, 'clipped')
+    assert flat[0] == before[0]
+
+
+def test_many_small_tensors():
+    """more partials than a workgroup of the scaling reads by itself, in a list that a cache holds"""
+    from rtg import ops
+    ts = gradients([50 + i % 11 for i in range(5000)], [F32, BF], 8, True)
+    before, norm = [t.clone() for t in ts], norm64(ts)
+    close(ops.clip_grads_(ts, 0.3 * norm), norm)
+    f = 0.3 * norm / (norm + 1e-6)
+    for kind in (F32, BF):
+        got, want = (torch.cat([t for t in l if t.dtype == kind]).double() for l in (ts, before))
+        inside(got, want * f, (2 * U + half_step(kind) + 1e-9) * want.abs() + 1e-40, 'clipped')
+
+
 def test_memory_around_the_tensors_is_left_alone():
     from rtg import ops
     for kind in (F32, BF):
@@ -269,6 +299,17 @@ def test_update(sizes, limit, off):
     verify(s, norm, want, update(s, limit * norm))
 
 
+def test_update_of_gradients_that_no_cache_holds():
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    sizes = [70_000_001, 5]
+    s = {k: [sc * torch.randn(n, generator=gen, device=DEV) for n in sizes] for k, sc in (('p', 0.5), ('g', 0.1), ('m', 0.05), ('v', 0.01))}
+    s['v'] = [t.abs() for t in s['v']]
+    s['t'] = [torch.full((1,), 4.0, device=DEV) for _ in sizes]
+    limit = 0.4 * norm64(s['g'])
+    norm, want = want64(s, limit)
+    verify(s, norm, want, update(s, limit))
+
+
 def test_without_a_limit_it_is_the_update_that_was_there():
     from rtg.lib import lib, check, current_stream_ptr
     from rtg.ops import _p
@@ -320,7 +361,7 @@ def test_adamw_refusals():
         with pytest.raises(RtgError):
             ops.clipped_adamw_(*cols, 1.0)
     for kw in ({'grad_scale': 0.0}, {'grad_scale': -1.0}, {'loss_flags': []}, {'loss_flags': [torch.zeros(2, device=DEV)]},
-               {'out': torch.zeros(2, device=DEV)}):
+               {'out': torch.zeros(2, device=DEV)}, {'out': t[0]}, {'out': m[0][7:8]}):
         with pytest.raises(RtgError):
             update(s, 1.0, **kw)
     for limit in (-1.0, float('nan')):

@@ -265,6 +265,17 @@ def test_offsets_past_32_bits():
         check(x, w, b, make(size, torch.bfloat16, 7, 0.0), dim)
 
 
+@pytest.mark.parametrize('shape,dim,kind', [((16_500, 4099), -1, torch.float32), ((270_001, 250), -1, torch.float32), ((530_001, 260), -1, torch.bfloat16),
+                                            ((4200, 16_390), -1, torch.float32), ((32, 129, 16_390), 1, torch.float32), ((16, 512, 8200), 1, torch.float32),
+                                            ((33, 100, 41_000), 1, torch.bfloat16)])
+def test_activations_that_no_cache_holds(shape, dim, kind):
+    """256 MB and more, which are read past the caches"""
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    x, dy = (torch.randn(shape, generator=gen, device=DEV).add_(level).to(kind) for level in (1.0, 0.0))
+    assert x.numel() * x.element_size() >= 256 << 20
+    check(x, *params(shape[dim], torch.float32, 9), dy, dim)
+
+
 def test_another_stream():
     from rtg import ops
     x, w, b = make((64, 1000), torch.float32, 1), *params(1000, torch.float32, 2)

@@ -1502,7 +1502,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
     bfloat16, taken as the values it holds (a bf16 map of the discriminators goes through ops.decode first); weight / bias:
     float32 or bfloat16 of shape (n,), or None.  Strided rows, time crops and channel slices of a map are read in place, and a
     map whose channels are adjacent ([B, T, C] transposed) takes the row kernels; the result is as dense as x is.  One launch
-    forward, two backward (gradients of x, weight and bias, summed in a fixed order); not differentiable twice."""
+    forward, two backward (gradients of x, weight and bias, summed in a fixed order); not differentiable twice.  A backward pass
+    that is captured into a graph must not meet an eager autograd graph of the same leaves that is still alive (autograd's own
+    rule): drop that one first, or capture layer_norm_forward and layer_norm_backward, which have none."""
     p = _norm_call(x, weight, bias, eps, dim)
     if p.as_rows:
         return layer_norm(x.movedim(p.dim, -1), weight, bias, eps, -1).movedim(-1, p.dim)
@@ -1539,6 +1541,7 @@ def _limit(max_norm):
     return float(max_norm)
 
 
+_MOST_TENSORS = 1 << 20
 _TB = torch._C.TensorBase
 _dtype_of = operator.attrgetter('dtype')
 
@@ -1551,6 +1554,8 @@ class _GradList:
         ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
         if not ts:
             raise L.RtgError(f'{what}: no gradients')
+        if len(ts) > _MOST_TENSORS:
+            raise L.RtgError(f'{what}: {len(ts)} gradients (at most {_MOST_TENSORS})')
         kinds = list(map(_dtype_of, ts))
         found = set(kinds)
         if not found.issubset(_NORM_TYPES):
@@ -1620,7 +1625,7 @@ def clipped_adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, max_norm, lr=1e-
     cols = [list(c) for c in (params, grads, exp_avgs, exp_avg_sqs, steps)]
     n = len(cols[0])
     flags = [None] * n if loss_flags is None else list(loss_flags)
-    if n < 1 or any(len(c) != n for c in cols) or len(flags) != n:
+    if not 1 <= n <= _MOST_TENSORS or any(len(c) != n for c in cols) or len(flags) != n:
         raise L.RtgError(f'clipped_adamw_: lists of {[len(c) for c in cols]} buffers and {len(flags)} loss flags')
     if not grad_scale > 0.0:
         raise L.RtgError(f'clipped_adamw_: grad_scale {grad_scale!r}')
