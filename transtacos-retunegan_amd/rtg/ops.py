@@ -1422,13 +1422,18 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _empty_as(t):
+    """contiguous, of t's shape and type (empty_like keeps the order of a permuted tensor, and is half the host time)"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
 def _norm_forward(x, weight, bias, eps, p, keep):
     """checked operands and their plan -> (y, statistics [mean | rstd] or None, x as read, the plan it was read with)"""
     if p.desc is None:
         like = weight if weight is not None else bias
         x, p = _norm_operands(x, None if like is None else like.dtype, eps, p.dim)
     weight, bias = _c(weight), _c(bias)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = _empty_as(x)
     stats = torch.empty(2 * p.rows, device=x.device) if keep else None
     mean = stats.data_ptr() if keep else None
     args = (p.ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean, mean + 4 * p.rows if keep else None, _stream())
@@ -1442,7 +1447,7 @@ def _norm_backward(dy, x, mean, rstd, weight, p, kind, needs):
     """mean, rstd: addresses; p: the plan of x with parameter gradients of type `kind`"""
     dy, weight = _c(dy), _c(weight)
     dev = x.device
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if needs[0] else None
+    dx = _empty_as(x) if needs[0] else None
     dw = torch.empty(p.n, device=dev, dtype=kind) if needs[1] else None
     db = torch.empty(p.n, device=dev, dtype=kind) if needs[2] else None
     ws = torch.empty(p.scratch(), device=dev) if needs[1] or needs[2] else None
