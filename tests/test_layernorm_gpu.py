@@ -265,6 +265,15 @@ def test_offsets_past_32_bits():
         check(x, w, b, make(size, torch.bfloat16, 7, 0.0), dim)
 
 
+def test_channels_far_apart():
+    """more than 2^24 elements between the channels of a map: the offsets inside a tile would pass 32 bits"""
+    for t in (70, 3):
+        size, stride = (2, 20, t), (t + 1, (1 << 24) + 3, 1)
+        x = torch.empty(20 * stride[1] + 4096, device=DEV, dtype=torch.bfloat16).as_strided(size, stride)
+        x.copy_(make(size, torch.bfloat16, 5))
+        check(x, *params(20, torch.float32, 6), make(size, torch.bfloat16, 7, 0.0), 1)
+
+
 @pytest.mark.parametrize('shape,dim,kind', [((16_500, 4099), -1, torch.float32), ((270_001, 250), -1, torch.float32), ((530_001, 260), -1, torch.bfloat16),
                                             ((4200, 16_390), -1, torch.float32), ((32, 129, 16_390), 1, torch.float32), ((16, 512, 8200), 1, torch.float32),
                                             ((33, 100, 41_000), 1, torch.bfloat16)])
