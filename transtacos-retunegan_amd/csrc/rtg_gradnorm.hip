@@ -505,9 +505,11 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
   const float w1 = (float)(1.0 - beta1), w2 = (float)(1.0 - beta2), decay = (float)(1.0 - lr * weight_decay);
   AdamScalars* sc = reinterpret_cast<AdamScalars*>(ws + MOST_CHUNKS + n);
   const long long chunk = chunk_bytes(4 * total);
-  // (the update in smaller pieces than the norm: four streams in, three out, and no partial a piece: 27 M parameters 172 us, in
-  // the norm's 181)
-  const long long piece = up(4 * total / MOST_CHUNKS);
+  // The update in smaller pieces than the norm: four streams in, three out, and no partial a piece.  A vector of each a thread
+  // (27 M parameters 143 us, in pieces of 16 KB 147; 84 M 413 and 431, in 8192 pieces 454); where every workgroup joins the
+  // partials first, four, but a workgroup for each CU where there is that much (2.7 M 21.1 us, in pieces of 4 KB 24.7; 0.2 M
+  // 9.7 and 8.2).
+  const long long least = up(total >> 18), few = up(total >> 6);
   AdamTable a;
   const auto fill = [&](int from, long long bytes) {           // -> workgroups
     int here = 0;
@@ -524,12 +526,13 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
     RTG_KLAUNCH(adam_partial, dim3(blocks), dim3(THREADS), 0, st, a, ws, sc);
     const int rc = rtg_launch_status();
     if (rc != RTG_OK) return rc;
-    const int here = fill(0, piece < 16384 ? 16384 : piece);
+    const int here = fill(0, few < 4096 ? 4096 : few > 16384 ? 16384 : few);
     RTG_KLAUNCH(adam_update<true>, dim3(here), dim3(THREADS), 0, st, a, (const AdamScalars*)sc, (const double*)ws, blocks, rates, norm_out,
                 w1, (float)beta2, w2, decay, (float)eps);
     return rtg_launch_status();
   }
-  // the partials, TABLE buffers a launch
+  // the partials, TABLE buffers a launch (in the caches whatever their size: the update reads past them, and a part stays: 84 M
+  // parameters 491 -> 454 us)
   GradTable t;
   t.chunk = chunk;
   for (int k = 0; k < TABLE / 32; ++k) t.bf16[k] = 0;
@@ -543,14 +546,13 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
       t.first[t.count] = here;
       here += (int)((4 * j.n + t.chunk - 1) / t.chunk);
     }
-    if (4 * total > CACHED) RTG_KLAUNCH((grad_partial<RTG_NORM_L2, true>), dim3(here), dim3(THREADS), 0, st, t, ws + blocks);
-    else RTG_KLAUNCH((grad_partial<RTG_NORM_L2, false>), dim3(here), dim3(THREADS), 0, st, t, ws + blocks);
+    RTG_KLAUNCH((grad_partial<RTG_NORM_L2, false>), dim3(here), dim3(THREADS), 0, st, t, ws + blocks);
     const int rc = rtg_launch_status();
     if (rc != RTG_OK) return rc;
     blocks += here;
   }
   for (int i = 0; i < n; i += JOBS) {
-    const int here = fill(i, piece < 16384 ? 16384 : piece);
+    const int here = fill(i, least < 4096 ? 4096 : least);
     RTG_KLAUNCH(adam_prepare, dim3(1), dim3(REDUCE), 0, st, a, (const double*)ws, blocks, rates, sc + i, norm_out, (int)(i == 0));
     int rc = rtg_launch_status();
     if (rc != RTG_OK) return rc;
