@@ -4,8 +4,9 @@
 //   norm = sqrt(sum_t sum_i g_t[i]^2)  or  max |g|;   factor = min(1, max_norm / (norm + 1e-6))
 //
 // One multiply-add per element of 2 or 4 bytes: bound by HBM (and, for a small model, by the launches).  The tensors are cut
-// into chunks of one size, a workgroup each, whatever their number: 172 tensors of a generator are one launch.  A chunk's sum
-// is a double: the square of any float is a normal double, so nothing overflows or vanishes, and the result does not depend
+// into chunks of one size, whatever their number: 172 tensors of a generator are one launch.  A workgroup takes every so many-th
+// chunk, so that all of them together walk the list from its start to its end (adjacent pages of HBM at any one time: 134 M
+// floats clipped in 278 us, with one long chunk a workgroup 296).  A workgroup's sum is a double: the square of any float is a normal double, so nothing overflows or vanishes, and the result does not depend
 // on how a list is cut into tensors beyond the last bits of a double.
 #include "rtg_vec.h"
 #include <algorithm>
@@ -22,9 +23,9 @@ constexpr int REDUCE = 1024;
 struct GradTable {
   void* p[TABLE];
   long long n[TABLE];
-  int first[TABLE];                   // first workgroup of tensor i in this launch (increasing; empty tensors have none)
+  int first[TABLE];                   // first chunk of tensor i in this launch (increasing; empty tensors have none)
   unsigned bf16[TABLE / 32];
-  int count;
+  int count, chunks;
   long long chunk;                    // bytes of a chunk, a multiple of 4096
 };
 
@@ -126,14 +127,14 @@ __device__ __forceinline__ double chunk_sum(const T* __restrict__ p, long long n
   return join<KIND>(join<KIND>(acc[0], acc[1]), join<KIND>(acc[2], acc[3]));
 }
 
-// what workgroup blockIdx.x covers: [lo, lo + n) of entry i
+// chunk b: [lo, lo + n) of entry i
 struct Piece { int i; long long lo, n; bool bf; };
-__device__ __forceinline__ Piece piece_of(const GradTable& t) {
+__device__ __forceinline__ Piece piece_of(const GradTable& t, int b) {
   Piece r;
-  r.i = entry_of(t.first, t.count, blockIdx.x);
+  r.i = entry_of(t.first, t.count, b);
   r.bf = (t.bf16[r.i >> 5] >> (r.i & 31)) & 1;
   const long long size = t.chunk >> (r.bf ? 1 : 2);
-  r.lo = (long long)((int)blockIdx.x - t.first[r.i]) * size;
+  r.lo = (long long)(b - t.first[r.i]) * size;
   const long long left = t.n[r.i] - r.lo;
   r.n = left < size ? left : size;
   return r;
@@ -141,17 +142,22 @@ __device__ __forceinline__ Piece piece_of(const GradTable& t) {
 
 // Who reads a tensor again, and from where: a list of up to CACHED bytes is still in the memory-side cache (256 MB) when the
 // scaling or the update comes, so its norm leaves it there and the scaling, its last reader, makes no room for what it reads and
-// writes (27 M floats clipped 69.5 -> 62.0 us; with both passes that way 74, the second then reads HBM).  Of a longer list
-// nothing is left by then: its norm reads past the caches (1 GB of bf16 204 -> 187 us, 5.75 TB/s; clipped 678 -> 623).
+// writes (27 M floats clipped in 58 us; with plain accesses 8 more, with both passes that way 12: the second then reads HBM).  Of
+// a longer list nothing is left by then: its norm reads past the caches (1 GB of bf16 184 us, 5.8 TB/s, with plain reads 17
+// more; clipped 591 and 55 more).
 constexpr long long CACHED = 256ll << 20;
 
 template <int KIND, bool ONCE>
 __global__ __launch_bounds__(THREADS) void grad_partial(const GradTable t, double* __restrict__ part) {
   __shared__ double red[THREADS / 64];
-  const Piece c = piece_of(t);
-  double acc;
-  if (c.bf) acc = chunk_sum<rtg_bf16, KIND, ONCE>(reinterpret_cast<const rtg_bf16*>(t.p[c.i]) + c.lo, c.n);
-  else acc = chunk_sum<float, KIND, ONCE>(reinterpret_cast<const float*>(t.p[c.i]) + c.lo, c.n);
+  double acc = 0.0;
+  for (int b = blockIdx.x; b < t.chunks; b += gridDim.x) {
+    const Piece c = piece_of(t, b);
+    double sum;
+    if (c.bf) sum = chunk_sum<rtg_bf16, KIND, ONCE>(reinterpret_cast<const rtg_bf16*>(t.p[c.i]) + c.lo, c.n);
+    else sum = chunk_sum<float, KIND, ONCE>(reinterpret_cast<const float*>(t.p[c.i]) + c.lo, c.n);
+    acc = join<KIND>(acc, sum);
+  }
   acc = block_join<KIND, THREADS>(acc, red);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
@@ -197,9 +203,11 @@ __global__ __launch_bounds__(THREADS) void grad_scale(const GradTable t, const d
   if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *out = (float)norm;
   const float f = clip_factor(norm, max_norm);
   if (f == 1.f) return;
-  const Piece c = piece_of(t);
-  if (c.bf) chunk_scale<rtg_bf16, ONCE>(reinterpret_cast<rtg_bf16*>(t.p[c.i]) + c.lo, c.n, f);
-  else chunk_scale<float, ONCE>(reinterpret_cast<float*>(t.p[c.i]) + c.lo, c.n, f);
+  for (int b = blockIdx.x; b < t.chunks; b += gridDim.x) {
+    const Piece c = piece_of(t, b);
+    if (c.bf) chunk_scale<rtg_bf16, ONCE>(reinterpret_cast<rtg_bf16*>(t.p[c.i]) + c.lo, c.n, f);
+    else chunk_scale<float, ONCE>(reinterpret_cast<float*>(t.p[c.i]) + c.lo, c.n, f);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -244,7 +252,7 @@ __global__ __launch_bounds__(REDUCE) void adam_prepare(const AdamTable t, const 
 
 // Few of them: the partial sums carry the counters and flags as they were (`held`), so that every workgroup of the update makes
 // the scalars itself and one of them may advance the counter at once: two launches (2.7 M parameters 22.4 -> 21.2 us, 1000 parameters 8.4 -> 6.6)
-constexpr int FEW_PARTIALS = 1024;
+constexpr long long FEW_BYTES = 16ll << 20;
 __global__ __launch_bounds__(THREADS) void adam_partial(const AdamTable t, double* __restrict__ part, AdamScalars* __restrict__ held) {
   __shared__ double red[THREADS / 64];
   const int j = entry_of(t.first, t.count, blockIdx.x);
@@ -258,8 +266,8 @@ __global__ __launch_bounds__(THREADS) void adam_partial(const AdamTable t, doubl
 
 // FEW: sc is what adam_partial held; else what adam_prepare made.  Parameters, gradients and moments pass the caches by where
 // they are many: what the memory-side cache holds is then the gradients that the norm has just read, not the moments of
-// buffers that are done with until the next step (27 M parameters 175 -> 149 us); a small model fits as a whole (2.7 M: 22.6
-// either way).
+// buffers that are done with until the next step (27 M parameters 139 us, with plain accesses 26 more).  A small model may fit as
+// a whole (2.7 M in the caches 21.1 us, past them 23.6; coming from HBM 26.1 and 23.9).
 template <bool FEW>
 __global__ __launch_bounds__(THREADS) void adam_update(const AdamTable t, const AdamScalars* __restrict__ sc, const double* __restrict__ part,
                                                        int n_part, const AdamRates rates, float* __restrict__ norm_out, float w1, float b2,
@@ -320,14 +328,17 @@ __global__ __launch_bounds__(THREADS) void adam_update(const AdamTable t, const 
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int MAX_TENSORS = 1 << 20;
 
-// Bytes of a chunk: 2048 chunks (8 workgroups a CU) of 16 to 256 KB each, more of 256 KB where that many do not hold the list
-// (an even end: 1 GB in 2048 chunks 251 us, in 4096 230 us; 110 MB 27 and 28 us), but no more than 8192: the clipping kernels
-// read every partial in every workgroup.
-constexpr int MOST_CHUNKS = 8192;
+constexpr int MOST_GROUPS = 4096;
+constexpr long long KB = 1024;
 long long up(long long bytes) { return (bytes + 4095) / 4096 * 4096; }
-long long chunk_bytes(long long total) {
-  const long long even = up(total / 2048), c = even < 16384 ? 16384 : even > 262144 ? 262144 : even, least = up(total / MOST_CHUNKS);
-  return c > least ? c : least;
+
+// Bytes of a chunk, and the workgroups that share a launch's chunks (8 a CU, 16 where the list is not in the caches).  Norm /
+// clipping of 27 M floats with chunks of 16, 32, 64 KB: 28.4 / 59.7, 25.5 / 57.7, 26.0 / 61.1 us; of 2.7 M 9.7 / 16.0, 9.9 / 16.0,
+// 10.4 / 17.4; of 537 M bf16 values in 4096 workgroups 207 / 609, 189 / 585, 185 / 591, in 2048 241 / 655, 214 / 621, 203 / 618.
+struct Cut { long long chunk; int groups; };
+Cut cut_of(long long total) {
+  const long long c = total < 32 * KB * KB ? 16 * KB : total <= CACHED ? 32 * KB : 64 * KB, least = up(total >> 20);
+  return {c > least ? c : least, total <= CACHED ? MOST_GROUPS / 2 : MOST_GROUPS};
 }
 
 long long list_bytes(int n, const long long* counts, const int* bf16) {
@@ -337,15 +348,19 @@ long long list_bytes(int n, const long long* counts, const int* bf16) {
 }
 
 // walks the list, TABLE tensors a launch: launch(table, workgroups, workgroups before) for each -> status; *blocks: all of them
+// (at most MOST_GROUPS a launch)
 template <class F>
 int each_table(int n, void* const* grads, const long long* counts, const int* bf16, long long total, int* blocks, F launch) {
+  const Cut cut = cut_of(total);
   GradTable t;
-  t.chunk = chunk_bytes(total);
+  t.chunk = cut.chunk;
   int before = 0, here = 0;
   t.count = 0;
   for (int k = 0; k < TABLE / 32; ++k) t.bf16[k] = 0;
   for (int i = 0; i <= n; ++i) {
     if (t.count == TABLE || (i == n && t.count > 0)) {
+      t.chunks = here;
+      if (here > cut.groups) here = cut.groups;
       const int rc = launch(t, here, before);
       if (rc != RTG_OK) return rc;
       before += here;
@@ -432,12 +447,14 @@ int clip(int n, void* const* grads, const long long* counts, const int* bf16, do
   });
 }
 
+long long most_partials(int n) { return (long long)MOST_GROUPS * ((n + TABLE - 1) / TABLE); }
+
 }  // namespace
 
 extern "C" long long rtg_grad_ws(int n) {
   if (n < 1 || n > MAX_TENSORS) return RTG_EINVAL;
-  // a partial per chunk (at most MOST_CHUNKS full ones and a last one per tensor), and AdamW's scalars
-  return (long long)MOST_CHUNKS + n + (long long)n * (sizeof(AdamScalars) / sizeof(double));
+  // a partial per workgroup, and AdamW's scalars
+  return most_partials(n) + (long long)n * (sizeof(AdamScalars) / sizeof(double));
 }
 
 extern "C" int rtg_grad_norm(int n, const void* const* grads, const long long* counts, const int* bf16, int kind, double* ws,
@@ -503,8 +520,8 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
   hipStream_t st = (hipStream_t)stream;
   const AdamRates rates{max_norm, lr, beta1, beta2, grad_scale};
   const float w1 = (float)(1.0 - beta1), w2 = (float)(1.0 - beta2), decay = (float)(1.0 - lr * weight_decay);
-  AdamScalars* sc = reinterpret_cast<AdamScalars*>(ws + MOST_CHUNKS + n);
-  const long long chunk = chunk_bytes(4 * total);
+  AdamScalars* sc = reinterpret_cast<AdamScalars*>(ws + most_partials(n));
+  const Cut cut = cut_of(4 * total);
   // The update in smaller pieces than the norm: four streams in, three out, and no partial a piece.  A vector of each a thread
   // (27 M parameters 143 us, in pieces of 16 KB 147; 84 M 413 and 431, in 8192 pieces 454); where every workgroup joins the
   // partials first, four, but a workgroup for each CU where there is that much (2.7 M 21.1 us, in pieces of 4 KB 24.7; 0.2 M
@@ -521,8 +538,8 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
     }
     return here;
   };
-  int blocks = n <= JOBS ? fill(0, chunk) : FEW_PARTIALS + 1;
-  if (blocks <= FEW_PARTIALS) {
+  if (n <= JOBS && 4 * total <= FEW_BYTES) {
+    const int blocks = fill(0, cut.chunk);
     RTG_KLAUNCH(adam_partial, dim3(blocks), dim3(THREADS), 0, st, a, ws, sc);
     const int rc = rtg_launch_status();
     if (rc != RTG_OK) return rc;
@@ -534,9 +551,9 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
   // the partials, TABLE buffers a launch (in the caches whatever their size: the update reads past them, and a part stays: 84 M
   // parameters 491 -> 454 us)
   GradTable t;
-  t.chunk = chunk;
+  t.chunk = cut.chunk;
   for (int k = 0; k < TABLE / 32; ++k) t.bf16[k] = 0;
-  blocks = 0;
+  int blocks = 0;
   for (int i = 0; i < n; i += TABLE) {
     int here = 0;
     for (t.count = 0; t.count < TABLE && i + t.count < n; ++t.count) {
@@ -546,6 +563,8 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
       t.first[t.count] = here;
       here += (int)((4 * j.n + t.chunk - 1) / t.chunk);
     }
+    t.chunks = here;
+    if (here > cut.groups) here = cut.groups;
     RTG_KLAUNCH((grad_partial<RTG_NORM_L2, false>), dim3(here), dim3(THREADS), 0, st, t, ws + blocks);
     const int rc = rtg_launch_status();
     if (rc != RTG_OK) return rc;
