@@ -126,3 +126,17 @@ def test_the_reference_is_layer_norm_and_its_bounds_hold_for_a_float_evaluation(
     wrong = (xf - xf.mean(2, keepdim=True)) / (xf.var(2, keepdim=True) + 1e-5).sqrt() * w + b
     with pytest.raises(AssertionError):
         inside(wrong.transpose(1, 2).to(torch.float32 if kind == torch.float32 else kind), ref.y, ref.y_off, 'y')
+
+
+def test_backward_passes_stay_on_the_calling_thread():
+    """unless RTG_AUTOGRAD_THREADS=1 asks for autograd's own threads"""
+    import os
+    import subprocess
+    import sys
+    code = ("import importlib; importlib.import_module('transtacos-retunegan_amd'); from rtg import ops; import torch; "
+            "print(torch._C._is_multithreading_enabled())")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for value, want in (('0', 'False'), ('1', 'True')):
+        out = subprocess.run([sys.executable, '-c', code], cwd=root, env={**os.environ, 'RTG_AUTOGRAD_THREADS': value}, capture_output=True,
+                             text=True, check=True)
+        assert out.stdout.split()[-1] == want

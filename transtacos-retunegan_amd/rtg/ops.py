@@ -8,10 +8,14 @@ import os as _os
 
 import torch
 
+from . import config
 from . import lib as L
 from . import tune
 from . import bank as _bank
 from .lib import lib, check, current_stream_ptr as _lib_stream_ptr
+
+if config.get('RTG_AUTOGRAD_THREADS') == '0':
+    torch.autograd.set_multithreading_enabled(False)            # (of the importing thread; rtg/config.py has the reason)
 
 
 def _stream():
