@@ -4,7 +4,9 @@
 //   y = (x - mean) * rstd * w + b                                    per row: mean, var over n elements
 //   g = dy * w;  dx = rstd * (g - mean(g) - xhat * mean(g * xhat));  dw = sum dy * xhat;  db = sum dy
 //
-// ~8 (forward) and ~16 (backward) operations per element of 4 .. 12 bytes moved: bound by HBM.
+// ~8 (forward) and ~16 (backward) operations per element of 4 .. 12 bytes moved: bound by HBM, which the large problems reach:
+// 16384 x 4096 bf16 45.8 us forward (5.9 TB/s) and 75 backward (5.4), floats 83 (6.5) and 129 (6.2); a map of (32, 128, 16384)
+// floats 83 and 144; a token's row of 4096 3.4 us and a launch of nothing 2.8.
 #include "rtg_vec.h"
 
 namespace {
@@ -329,7 +331,8 @@ __global__ __launch_bounds__(BLK) void ln_row_bwd(LnShape s, const T* __restrict
 // ---------------------------------------------------------------------------------------------------------------------
 // Feature maps.  A wave holds a tile of LP * N adjacent positions (N in a lane's vector) with its 64 / LP channel lanes times
 // CPT channels each in registers; W waves share the channels of a tile where one cannot hold them.  Every load is a whole
-// 16 * LP bytes of a channel's row, CPT of them in flight per lane.
+// 16 * LP bytes of a channel's row, CPT of them in flight per lane: (32, 128, 2048) floats 12.0 us forward (5.6 TB/s), 24 backward;
+// (16, 512, 1025), whose channels start anywhere in a line, 14.6 and 34.5.
 // ---------------------------------------------------------------------------------------------------------------------
 // workgroup b of a grid of 8 k runs on XCD b % 8 (each has its own L2): neighbours in the order of the tiles are put on one XCD, so
 // a line that two tiles share — rows of a map that do not start on a line — is fetched once
@@ -591,7 +594,8 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* _
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Kernels for any size.  A row or a column of channels that no register kernel holds is read once per sum (the later reads
-// come from L2 or the memory-side cache): 1000 rows of 40000.  They also serve rows of less than a vector, a thread each.
+// come from L2 or the memory-side cache): 1000 rows of 40000 floats 97 us forward, 194 backward (3.3 and 2.5 TB/s of what has to
+// move).  They also serve rows of less than a vector, a thread each (1000000 x 5 floats 20 and 46 us).
 // ---------------------------------------------------------------------------------------------------------------------
 template <int BLK>
 __device__ __forceinline__ float loop_sum(float v, float* red) {
@@ -933,7 +937,8 @@ __global__ __launch_bounds__(TINY_THREADS) void ln_map_loop_dw(LnShape s, const 
 }
 
 // dw, db = the sums of their `slices` partials [slice][dw | db][n], each in the order of the slices: 32 columns a block, a
-// column's slices over 32 threads (so that the reads of a column are in flight together), then a fixed tree
+// column's slices over 32 threads (so that the reads of a column are in flight together), then a fixed tree: 256 partials of 2048
+// columns in 4 us
 __global__ __launch_bounds__(FIN_COLS* FIN_ROWS) void ln_finish(const float* __restrict__ part, int slices, long long n,
                                                                 void* __restrict__ dw, void* __restrict__ db, int pbf) {
   __shared__ float red[FIN_ROWS][FIN_COLS + 1];
@@ -996,8 +1001,9 @@ constexpr int LOOPS = -1, TINY = -2;
 // Rows: threads per row, 16-byte vectors per thread, threads per block.  Over 13 widths from 64 to 16384 and row counts from 1 to
 // 65536 these tiles are within 5 % of the best of 20 (forward) and 40 (backward); what they weigh: a wave's rows need no
 // barrier (up to two vectors a thread), a block's row two; the backward holds sixteen elements a thread at most (the weight, dw
-// and db take a register each); half the blocks that fit are enough where each walks its rows with the next in flight
-// (65536 x 1024 floats 91 us, with all of them 99).
+// and db take a register each).  Forward, as many blocks as fit up to 64 MB of rows (8192 x 2048 bf16 14.2 us, with half of them
+// 15.6; 4096 x 1024 floats 7.8 and 8.5; not of 1024 threads: 2048 x 16384 bf16 28.7 and 26.9), half of them beyond: each walks its rows with the next in flight, and fewer rows of
+// HBM are open at a time (65536 x 1024 floats 81 us, with all of them 83, with a quarter 110; 16384 x 4096 bf16 45.8, 48.6, 50.2).
 struct RowTile { int tpr, vpt, blk; };
 constexpr int ROW_TILES = 10;
 constexpr RowTile FWD_TILES[ROW_TILES] = {{8, 1, 256},   {16, 1, 256},  {32, 1, 256},  {64, 1, 256},   {64, 2, 256},
@@ -1102,7 +1108,9 @@ Plan plan_fwd(const RtgLayerNormDesc* d) {
     if (i == LOOPS) return {LOOPS, (int)lmin(d->outer, 1 << 20)};
     if (i == TINY) return {TINY, even_blocks((d->outer + TINY_THREADS - 1) / TINY_THREADS, 2048)};
     const int groups = FWD_TILES[i].blk / FWD_TILES[i].tpr;
-    return {i, even_blocks((d->outer + groups - 1) / groups, 256 * (1024 / FWD_TILES[i].blk))};
+    const bool all = d->outer * d->n * (d->bf16 ? 2 : 4) <= 64ll << 20 && FWD_TILES[i].blk < 1024;
+    const int threads = all ? 2048 : 1024;                 // a CU
+    return {i, even_blocks((d->outer + groups - 1) / groups, 256 * (threads / FWD_TILES[i].blk))};
   }
   const int key = map_fwd(d);
   const long long blocks = map_blocks(d, key);
