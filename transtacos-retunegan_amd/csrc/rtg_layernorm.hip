@@ -332,7 +332,7 @@ __global__ __launch_bounds__(BLK) void ln_row_bwd(LnShape s, const T* __restrict
 // Feature maps.  A wave holds a tile of LP * N adjacent positions (N in a lane's vector) with its 64 / LP channel lanes times
 // CPT channels each in registers; W waves share the channels of a tile where one cannot hold them.  Every load is a whole
 // 16 * LP bytes of a channel's row, CPT of them in flight per lane: (32, 128, 2048) floats 12.0 us forward (5.6 TB/s), 24 backward;
-// (16, 512, 1025), whose channels start anywhere in a line, 14.6 and 34.5.
+// (16, 512, 1025), whose channels start anywhere in a line, 14.6 and 31.5.
 // ---------------------------------------------------------------------------------------------------------------------
 // workgroup b of a grid of 8 k runs on XCD b % 8 (each has its own L2): neighbours in the order of the tiles are put on one XCD, so
 // a line that two tiles share — rows of a map that do not start on a line — is fetched once
@@ -1002,8 +1002,9 @@ constexpr int LOOPS = -1, TINY = -2;
 // 65536 these tiles are within 5 % of the best of 20 (forward) and 40 (backward); what they weigh: a wave's rows need no
 // barrier (up to two vectors a thread), a block's row two; the backward holds sixteen elements a thread at most (the weight, dw
 // and db take a register each).  Forward, as many blocks as fit up to 64 MB of rows (8192 x 2048 bf16 14.2 us, with half of them
-// 15.6; 4096 x 1024 floats 7.8 and 8.5; not of 1024 threads: 2048 x 16384 bf16 28.7 and 26.9), half of them beyond: each walks its rows with the next in flight, and fewer rows of
-// HBM are open at a time (65536 x 1024 floats 81 us, with all of them 83, with a quarter 110; 16384 x 4096 bf16 45.8, 48.6, 50.2).
+// 15.6; 4096 x 1024 floats 7.8 and 8.5; not of 1024 threads: 2048 x 16384 bf16 28.7 and 26.9), half of them beyond: each walks its
+// rows with the next in flight, and fewer rows of HBM are open at a time (65536 x 1024 floats 81 us, with all of them 83, with a
+// quarter 110; 16384 x 4096 bf16 45.8, 48.6, 50.2).
 struct RowTile { int tpr, vpt, blk; };
 constexpr int ROW_TILES = 10;
 constexpr RowTile FWD_TILES[ROW_TILES] = {{8, 1, 256},   {16, 1, 256},  {32, 1, 256},  {64, 1, 256},   {64, 2, 256},
@@ -1083,7 +1084,7 @@ int map_bwd(const RtgLayerNormDesc* d) {
   if (n <= 64) return map_key(8, 2, 4);
   if (n <= 128) return map_wide(d, 8, 1) ? map_key(8, 2, 8) : map_key(8, 4, 4);
   if (n <= 256) return map_wide(d, 8, 8) ? map_key(8, 8, 4) : map_key(4, 4, 4);
-  if (n <= 512) return map_wide(d, 8, 2) ? map_key(8, 8, 8) : map_key(4, 8, 4);
+  if (n <= 512) return map_wide(d, 8, 4) ? map_key(8, 8, 8) : map_key(4, 8, 4);
   if (n <= 1024) return map_wide(d, 4, 8) ? map_key(4, 8, 8) : map_key(2, 8, 4);
   return map_key(2, 16, 4);
 }
