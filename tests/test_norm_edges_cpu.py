@@ -1,0 +1,80 @@
+"""Calls of layer norm and of the gradient operators that lie beside the ordinary ones, as far as a machine without a GPU shows
+them: the launches are replaced by functions that look at what they are given."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+class Launches:
+    """stands in for the library: keeps the description and the address of each layer norm backward launch"""
+
+    def __init__(self):
+        self.backward = []
+
+    def rtg_layernorm_forward(self, *args):
+        return 0
+
+    def rtg_layernorm_ws(self, ref):
+        return 16
+
+    def rtg_layernorm_backward(self, ref, dy, x, *args):
+        d = ref._obj
+        self.backward.append(((d.outer, d.n, d.inner, d.x_outer, d.x_n), x))
+        return 0
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    from rtg import ops
+    fake = Launches()
+    monkeypatch.setattr(ops, 'lib', fake)
+    monkeypatch.setattr(ops, '_stream', lambda: None)
+    return fake
+
+
+def apply(x, w, b, dim):
+    from rtg import ops
+    return ops.LayerNormFn.apply(x, w, b, 1e-5, ops._norm_plan(x.shape, x.stride(), dim, x.dtype is torch.bfloat16, False, 1e-5))
+
+
+VIEWS = {'time crop': (lambda t: t[:, :, 5:44], 1), 'channel slice': (lambda t: t[:, 7:30], 1), 'row slice': (lambda t: t[:, :, 3:67], 2),
+         'last rows': (lambda t: t[:, -1], 1), 'whole': (lambda t: t, 1), 'every second': (lambda t: t[:, :, ::2], 1)}
+
+
+@pytest.mark.parametrize('view', list(VIEWS))
+def test_saved_activations_that_come_back_in_another_layout(launches, view):
+    """a saved-tensor hook may give the values back dense: what the backward launch reads has to lie where the tensor is"""
+    cut, dim = VIEWS[view]
+    base = torch.randn(4, 64, 200)
+    x = cut(base).requires_grad_(True)
+    w, b = torch.ones(x.shape[dim], requires_grad=True), torch.zeros(x.shape[dim], requires_grad=True)
+    back = []
+
+    def unpack(t):
+        back.append(t.float())
+        return back[-1]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.double().contiguous(), unpack):
+        y = apply(x, w, b, dim)
+    torch.autograd.grad(y, (x, w, b), torch.ones(x.shape))
+    saved = next(t for t in back if t.shape == x.shape)
+    (outer, n, inner, x_outer, x_n), at = launches.backward[-1]
+    assert (outer * n * inner, n, at) == (x.numel(), x.shape[dim], saved.data_ptr())
+    last = (outer - 1) * x_outer + (n - 1) * x_n + inner - 1
+    assert last == saved.numel() - 1 == saved.untyped_storage().nbytes() // 4 - 1, 'the launch reads behind the tensor'
+    # ... and without a hook it is read in place, where it can be
+    torch.autograd.grad(apply(x, w, b, dim), (x, w, b), torch.ones(x.shape))
+    assert (launches.backward[-1][1] == x.data_ptr()) == (view != 'every second')
+
+
+def test_saved_tensors_that_come_back_as_others_are_refused(launches):
+    from rtg.lib import RtgError
+    x, w = torch.randn(6, 16, requires_grad=True), torch.ones(16, requires_grad=True)
+    for what, other in (('activations', lambda t: t[:3] if t.dim() == 2 else t), ('activations', lambda t: t.double() if t.dim() == 2 else t),
+                        ('weight', lambda t: t[:8] if t.shape == (16,) else t), ('weight', lambda t: t.bfloat16() if t.shape == (16,) else t),
+                        ('statistics', lambda t: t[:6] if t.shape == (12,) else t)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), other):
+            y = apply(x, w, None, 1)
+        with pytest.raises(RtgError, match=what):
+            torch.autograd.grad(y, (x, w), torch.ones(6, 16))
+    assert not launches.backward

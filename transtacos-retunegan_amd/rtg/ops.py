@@ -1485,20 +1485,40 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, dim=-1, needs=(True, Tru
     return _norm_backward(dy, x, mean.data_ptr(), rstd.data_ptr(), weight, p, kind, needs)
 
 
+def _same(what, t, shape, kind, device):
+    if t.shape != shape or t.dtype is not kind or t.get_device() != device:
+        raise L.RtgError(f'layer_norm backward: a saved-tensor hook returned {what} of {t.dtype} {tuple(t.shape)} on {t.device}, expected '
+                         f'{kind} {tuple(shape)} on device {device}')
+
+
 class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, plan):
         y, stats, x, ctx.plan = _norm_forward(x, weight, bias, eps, plan, True)
         ctx.save_for_backward(x, weight, stats)
+        ctx.strides = x.stride()
         ctx.kind = weight.dtype if weight is not None else (torch.float32 if bias is None else bias.dtype)
         return y
+
+    @staticmethod
+    def restored(ctx, dy):
+        """the saved tensors and the plan to read them with.  A saved-tensor hook (torch.autograd.graph.save_on_cpu, a
+        checkpoint) may bring them back in another layout: activations with gaps come back dense"""
+        x, weight, stats = ctx.saved_tensors
+        p, here = ctx.plan, dy.get_device()
+        _same('activations', x, dy.shape, dy.dtype, here)
+        if x.stride() != ctx.strides:
+            x, p = _norm_operands(x, ctx.kind, 0.0, p.dim)
+        _same('statistics', stats, (2 * p.rows,), torch.float32, here)
+        if weight is not None:
+            _same('weight', weight, (p.n,), ctx.kind, here)
+        return x, weight, _c(stats), p
 
     @staticmethod
     def backward(ctx, dy):
         if torch.is_grad_enabled():                             # (create_graph: refuse to be differentiated once more)
             return LayerNormFn.once(ctx, dy)
-        x, weight, stats = ctx.saved_tensors
-        p = ctx.plan
+        x, weight, stats, p = LayerNormFn.restored(ctx, dy)
         mean = stats.data_ptr()
         return (*_norm_backward(dy, x, mean, mean + 4 * p.rows, weight, p, ctx.kind, ctx.needs_input_grad), None, None)
 
