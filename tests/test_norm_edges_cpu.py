@@ -78,3 +78,28 @@ def test_saved_tensors_that_come_back_as_others_are_refused(launches):
         with pytest.raises(RtgError, match=what):
             torch.autograd.grad(y, (x, w), torch.ones(6, 16))
     assert not launches.backward
+
+
+@pytest.mark.parametrize('which', [0, 1, 2])
+@pytest.mark.parametrize('wants_grad', [False, True])
+def test_forward_mode_tangents_are_refused(launches, monkeypatch, which, wants_grad):
+    """a dual operand's tangent would be lost without a word"""
+    import torch.autograd.forward_ad as fw
+    from rtg import ops
+    from rtg.lib import RtgError
+    monkeypatch.setattr(ops, '_need_here', lambda *a: None)
+    monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: -1)
+    ts = [torch.randn(4, 8).requires_grad_(wants_grad), torch.ones(8), torch.zeros(8)]
+    with fw.dual_level():
+        duals = list(ts)
+        duals[which] = fw.make_dual(ts[which], torch.ones_like(ts[which]))
+        for call in (ops.layer_norm, ops.layer_norm_forward):
+            with pytest.raises(RtgError, match='tangent'):
+                call(*duals)
+        if which < 2:
+            with pytest.raises(RtgError, match='tangent'):
+                ops.layer_norm_backward(ts[0], duals[0], torch.zeros(4), torch.ones(4), duals[1])
+        assert ops.layer_norm(*ts).shape == (4, 8)              # operands without one are ordinary
+    from models.layers import LayerNorm
+    with pytest.raises((RtgError, RuntimeError)):
+        torch.func.jvp(LayerNorm(8, dim=-1), (torch.randn(4, 8),), (torch.ones(4, 8),))

@@ -42,3 +42,16 @@ def test_saved_tensors_that_leave_and_come_back(view, how, kind):
     inside(got[1], ref.dw, ref.dw_off, 'dweight')
     inside(got[2], ref.db, ref.db_off, 'dbias')
     assert torch.equal(got[0], want[0])                         # (an element's gradient does not go by the layout it is read from)
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    from rtg import ops
+    from rtg.lib import RtgError
+    x, (w, b) = make((4, 48), torch.float32, 1), params(48, torch.float32, 2)
+    want = ops.layer_norm(x, w, b)
+    with fw.dual_level():
+        assert torch.equal(ops.layer_norm(x, w, b), want)
+        for duals in ((fw.make_dual(x, x), w, b), (x, fw.make_dual(w, w), b), (x, w, fw.make_dual(b, b))):
+            with pytest.raises(RtgError, match='tangent'):
+                ops.layer_norm(*duals)

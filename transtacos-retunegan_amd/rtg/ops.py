@@ -7,6 +7,7 @@ import operator
 import os as _os
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import config
 from . import lib as L
@@ -1407,8 +1408,15 @@ def _looks(t):
     return None if t is None else (t.shape, t.dtype, t.get_device())
 
 
+def _no_tangents(*ts):
+    if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise L.RtgError('layer_norm: a dual tensor (forward-mode differentiation): its tangent would be dropped')
+
+
 def _norm_call(x, weight, bias, eps, dim):
     """the checks and the plan of a call; calls that look alike are checked once"""
+    if _forward_ad._current_level >= 0:
+        _no_tangents(x, weight, bias)
     here = x.get_device()
     key = (x.shape, x.stride(), x.dtype, here, _looks(weight), _looks(bias), eps, dim)
     p = _NORM_SEEN.get(key)
@@ -1472,6 +1480,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, dim=-1, keep=False):
 def layer_norm_backward(dy, x, mean, rstd, weight=None, dim=-1, needs=(True, True, True), param_dtype=None):
     """(dx, dweight, dbias) of layer_norm_forward(x, weight, bias, eps, dim, keep=True); `needs` says which are wanted (None in
     the place of the others).  The gradients of weight and bias have weight's type (param_dtype where there is no weight)."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents(dy, x, mean, rstd, weight)
     dim = _check_norm(x, weight, None, 0.0, dim)
     _need_here('layer_norm', dy, mean, rstd)
     kind = weight.dtype if weight is not None else (param_dtype or torch.float32)
@@ -1531,7 +1541,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, dim=-1):
     bfloat16, taken as the values it holds (a bf16 map of the discriminators goes through ops.decode first); weight / bias:
     float32 or bfloat16 of shape (n,), or None.  Strided rows, time crops and channel slices of a map are read in place, and a
     map whose channels are adjacent ([B, T, C] transposed) takes the row kernels; the result is as dense as x is.  One launch
-    forward, two backward (gradients of x, weight and bias, summed in a fixed order); not differentiable twice.  A backward pass
+    forward, two backward (gradients of x, weight and bias, summed in a fixed order); not differentiable twice, nor forward-mode.  A backward pass
     that is captured into a graph must not meet an eager autograd graph of the same leaves that is still alive (autograd's own
     rule): drop that one first, or capture layer_norm_forward and layer_norm_backward, which have none."""
     p = _norm_call(x, weight, bias, eps, dim)
