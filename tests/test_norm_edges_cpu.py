@@ -1,7 +1,5 @@
 """Calls of layer norm and of the gradient operators that lie beside the ordinary ones, as far as a machine without a GPU shows
 them: the launches are replaced by functions that look at what they are given."""
-import ctypes as C
-
 import pytest
 import torch
 
@@ -30,6 +28,7 @@ def launches(monkeypatch):
     fake = Launches()
     monkeypatch.setattr(ops, 'lib', fake)
     monkeypatch.setattr(ops, '_stream', lambda: None)
+    monkeypatch.setattr(ops, '_NORM_SEEN', {})
     return fake
 
 
