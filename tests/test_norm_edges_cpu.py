@@ -102,3 +102,16 @@ def test_forward_mode_tangents_are_refused(launches, monkeypatch, which, wants_g
     from models.layers import LayerNorm
     with pytest.raises((RtgError, RuntimeError)):
         torch.func.jvp(LayerNorm(8, dim=-1), (torch.randn(4, 8),), (torch.ones(4, 8),))
+
+
+def test_an_import_leaves_the_threads_of_autograd_alone():
+    """unless the program asks for its own thread (RTG_AUTOGRAD_THREADS=0)"""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch, importlib; before = torch._C._is_multithreading_enabled(); importlib.import_module('transtacos-retunegan_amd'); "
+            "from rtg import ops; import train, models; print(before, torch._C._is_multithreading_enabled())")
+    env = {k: v for k, v in os.environ.items() if k != 'RTG_AUTOGRAD_THREADS'}
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, '-c', code], cwd=root, env=env, capture_output=True, text=True, check=True)
+    assert out.stdout.split()[-2:] == ['True', 'True']

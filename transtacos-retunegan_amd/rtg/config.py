@@ -16,11 +16,12 @@ KNOBS = {
     'RTG_TEST_FAIL_CAPTURE': ('0', 'test hook: an illegal synchronous copy inside the capture (bench.py\'s eager fallback)'),
     'RTG_DEV_LIB': ('', 'path of a development build of librtg.so to load instead of the in-tree one (ablation builds)'),
     'RTG_EXTRA_FLAGS': ('', 'build.py: extra hipcc flags (ablation defines are refused there)'),
-    # one process drives one GPU: the backward pass runs on the thread that asks for it (torch.autograd.set_multithreading_enabled,
-    # set by rtg.ops for the thread that imports it).  On the engine's own thread for the device a pass waits for two threads to
-    # wake, and its allocations and launches work on the other core's cache lines: a layer norm's forward and backward 106 us of
-    # host time there, 46 on the calling thread
-    'RTG_AUTOGRAD_THREADS': ('0', '1: backward passes on autograd\'s thread for the device (torch\'s default)'),
+    # 0: rtg.ops switches autograd's threads off for the thread that imports it (torch.autograd.set_multithreading_enabled).  For a
+    # program that drives one GPU and has small backward passes: on the engine's own thread for the device a pass waits for two
+    # threads to wake, and its allocations work on the other core's cache lines (a layer norm's forward and backward 125 us of
+    # host time there, 57 on the calling thread).  It holds for every backward pass of that thread, and a program that drives
+    # several GPUs would run theirs one after the other, so it is the program's choice
+    'RTG_AUTOGRAD_THREADS': ('1', '0: backward passes on the thread that calls them instead of autograd\'s thread for the device (torch\'s default)'),
     # a switch of the HIP RUNTIME, not of this package: kernel arguments in device memory instead of host-coherent memory — the
     # command processor fetches them faster, which a step of 670 launches (115 of them one dependent chain) feels: round 6,
     # same-box A/B of the replayed config-2 step, four pairs: 26.35 / 26.43 / 26.55 / 26.42 ms with it, 26.72 / 26.65 / 26.85 /

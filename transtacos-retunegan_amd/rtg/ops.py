@@ -16,7 +16,7 @@ from . import bank as _bank
 from .lib import lib, check, current_stream_ptr as _lib_stream_ptr
 
 if config.get('RTG_AUTOGRAD_THREADS') == '0':
-    torch.autograd.set_multithreading_enabled(False)            # (of the importing thread; rtg/config.py has the reason)
+    torch.autograd.set_multithreading_enabled(False)            # (of the importing thread, where the program asks for it)
 
 
 def _stream():
