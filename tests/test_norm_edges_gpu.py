@@ -55,3 +55,42 @@ def test_forward_mode_tangents_are_refused():
         for duals in ((fw.make_dual(x, x), w, b), (x, fw.make_dual(w, w), b), (x, w, fw.make_dual(b, b))):
             with pytest.raises(RtgError, match='tangent'):
                 ops.layer_norm(*duals)
+
+
+@pytest.mark.parametrize('clips,n,t', [((1 << 26) + 5, 2, 2), ((1 << 24) + 3, 33, 2)])
+def test_more_tiles_than_a_launch_holds(clips, n, t):
+    """maps of many short clips: a block of 256 threads for every one or four of them would be 2^32 threads and more"""
+    from rtg import ops
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x, dy = (torch.empty(clips, n, t, device=DEV, dtype=torch.bfloat16).normal_(m, 1.0, generator=gen) for m in (1.0, 0.0))
+    w, b = params(n, torch.float32, 2)
+    y, mean, rstd = ops.layer_norm_forward(x, w, b, dim=1, keep=True)
+    dx, _, _ = ops.layer_norm_backward(dy, x, mean, rstd, w, dim=1, needs=(True, False, False))
+    for at in range(0, clips, 1 << 21):
+        cut = slice(at, min(at + (1 << 21), clips))
+        ref = Reference(x[cut], w, b, 1e-5).backward(dy[cut], torch.float32)
+        inside(y[cut], ref.y, ref.y_off, 'y')
+        inside(dx[cut], ref.dx, ref.dx_off, 'dx')
+
+
+@pytest.mark.parametrize('n', [(1 << 27) + 64, (1 << 30) + 256])
+def test_rows_longer_than_a_launch_has_threads(n):
+    """One row of +1, -1, ... with the gradient +2, +2, -2, -2, ...: sums of whole numbers that a float holds (n is a multiple of
+    its step there), so the mean and both sums of dx are 0, the variance is 1 up to the rounding of 1 / n, and
+    y = x, dx = dy, dweight = dy x up to the roundings of that and of the scale (u each, 8 in all)."""
+    from norm_reference import U
+    from rtg import ops
+    x = torch.tensor([1.0, -1.0], device=DEV).repeat(n // 2).view(1, n)
+    dy = torch.tensor([2.0, 2.0, -2.0, -2.0], device=DEV).repeat(n // 4).view(1, n)
+    y, mean, rstd = ops.layer_norm_forward(x, eps=0.0, keep=True)
+    assert mean.item() == 0.0 and abs(rstd.item() - 1.0) <= 4 * U
+    assert ((y - x).abs() <= 8 * U).all()
+    del y
+    dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd)
+    assert torch.equal(db, dy[0])
+    assert ((dx - dy).abs() <= 16 * U).all()
+    assert (dw.sub_(dy[0] * x[0]).abs_() <= 16 * U).all()
+    del dx, dw, db
+    empty = x[:0]
+    _, dw, db = ops.layer_norm_backward(empty, empty, mean[:0], rstd[:0])
+    assert dw.shape == db.shape == (n,) and not dw.any() and not db.any()

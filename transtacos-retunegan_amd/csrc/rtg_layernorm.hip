@@ -454,14 +454,15 @@ struct MapLane {
 template <class V, int LP, int W, int CPT, class T = typename V::T>
 __global__ __launch_bounds__(map_block(W)) void ln_map_fwd(LnShape s, const T* __restrict__ x, const void* __restrict__ w,
                                                                            const void* __restrict__ b, T* __restrict__ y,
-                                                                           float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+                                                                           float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                                                           unsigned first) {
   using M = MapTile<V, LP, W, CPT>;
   constexpr int N = M::N;
   constexpr int R = rtg_scattered(LP, N);
   __shared__ float red[2][W > 1 ? M::BLK / 64 : 1][64 * R];
   MapLane<V, LP, W, CPT> at(s);
   const unsigned per = (unsigned)((s.inner + M::POS - 1) / M::POS);
-  at.go(s, xcd_order(blockIdx.x, gridDim.x) * M::TEAMS + at.wave / W, (unsigned)s.outer * per, per);
+  at.go(s, (first + xcd_order(blockIdx.x, gridDim.x)) * M::TEAMS + at.wave / W, (unsigned)s.outer * per, per);
   V v[CPT];
   at.load(v, x, s.xo, s.xn, s.once);
   float wr[CPT], br[CPT], a[N], mean[N], rstd[N];
@@ -720,33 +721,35 @@ __global__ __launch_bounds__(LOOP_THREADS) void ln_row_loop_dw(LnShape s, const 
   constexpr int N = RtgVec<T>::N;
   __shared__ float red[DW_WAVES][64 * N];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long long i = ((long long)blockIdx.x * 64 + lane) * N, at = i < s.n - N ? i : s.n - N;      // (n >= N: ln_tiny has the rest)
-  float aw[N], ab[N];
+  for (long long c = (long long)blockIdx.x * 64 * N; c < s.n; c += (long long)gridDim.x * 64 * N) {
+    const long long i = c + lane * N, at = i < s.n - N ? i : s.n - N;                   // (n >= N: ln_tiny has the rest)
+    float aw[N], ab[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) aw[e] = ab[e] = 0.f;
-  for (long long row = blockIdx.y * DW_WAVES + wave; row < s.outer; row += (long long)DW_WAVES * slices) {
-    RtgVec<T> xv, gv;
-    xv.load(x + row * s.xo + at);
-    gv.load(dy + row * s.n + at);
-    const float m = mean[row], r = rstd[row];
+    for (int e = 0; e < N; ++e) aw[e] = ab[e] = 0.f;
+    for (long long row = blockIdx.y * DW_WAVES + wave; row < s.outer; row += (long long)DW_WAVES * slices) {
+      RtgVec<T> xv, gv;
+      xv.load(x + row * s.xo + at);
+      gv.load(dy + row * s.n + at);
+      const float m = mean[row], r = rstd[row];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      aw[e] += gv.get(e) * ((xv.get(e) - m) * r);
-      ab[e] += gv.get(e);
+      for (int e = 0; e < N; ++e) {
+        aw[e] += gv.get(e) * ((xv.get(e) - m) * r);
+        ab[e] += gv.get(e);
+      }
     }
-  }
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    __syncthreads();
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
 #pragma unroll
-    for (int e = 0; e < N; ++e) red[wave][lane * N + e] = which ? ab[e] : aw[e];
-    __syncthreads();
-    for (int j = threadIdx.x; j < 64 * N; j += LOOP_THREADS) {
-      const long long first = ((long long)blockIdx.x * 64 + j / N) * N, col = first < s.n - N ? first : s.n - N;
-      float v = 0.f;
+      for (int e = 0; e < N; ++e) red[wave][lane * N + e] = which ? ab[e] : aw[e];
+      __syncthreads();
+      for (int j = threadIdx.x; j < 64 * N; j += LOOP_THREADS) {
+        const long long first = c + j / N * N, col = first < s.n - N ? first : s.n - N;
+        float v = 0.f;
 #pragma unroll
-      for (int k = 0; k < DW_WAVES; ++k) v += red[k][j];
-      if (j % N >= first - col) part[((long long)blockIdx.y * 2 + which) * s.n + col + j % N] = v;
+        for (int k = 0; k < DW_WAVES; ++k) v += red[k][j];
+        if (j % N >= first - col) part[((long long)blockIdx.y * 2 + which) * s.n + col + j % N] = v;
+      }
     }
   }
 }
@@ -945,34 +948,41 @@ __global__ __launch_bounds__(FIN_COLS* FIN_ROWS) void ln_finish(const float* __r
   void* const out = blockIdx.y ? db : dw;
   if (!out) return;                                        // (the whole block)
   const int col = threadIdx.x % FIN_COLS, r = threadIdx.x / FIN_COLS;
-  const long long i = (long long)blockIdx.x * FIN_COLS + col;
-  float acc = 0.f;
-  if (i < n) {
-    const float* p = part + (long long)blockIdx.y * n + i;
-    int q = r;
-    for (; q + 7 * FIN_ROWS < slices; q += 8 * FIN_ROWS) {
-      float v[8];
+  for (long long c = (long long)blockIdx.x * FIN_COLS; c < n; c += (long long)gridDim.x * FIN_COLS) {
+    const long long i = c + col;
+    float acc = 0.f;
+    if (i < n) {
+      const float* p = part + (long long)blockIdx.y * n + i;
+      int q = r;
+      for (; q + 7 * FIN_ROWS < slices; q += 8 * FIN_ROWS) {
+        float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = p[(long long)(q + k * FIN_ROWS) * 2 * n];
+        for (int k = 0; k < 8; ++k) v[k] = p[(long long)(q + k * FIN_ROWS) * 2 * n];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) acc += v[k];
+        for (int k = 0; k < 8; ++k) acc += v[k];
+      }
+      for (; q < slices; q += FIN_ROWS) acc += p[(long long)q * 2 * n];
     }
-    for (; q < slices; q += FIN_ROWS) acc += p[(long long)q * 2 * n];
-  }
-  red[r][col] = acc;
-  __syncthreads();
-#pragma unroll
-  for (int h = FIN_ROWS / 2; h > 0; h >>= 1) {
-    if (r < h) red[r][col] += red[r + h][col];
+    red[r][col] = acc;
     __syncthreads();
+#pragma unroll
+    for (int h = FIN_ROWS / 2; h > 0; h >>= 1) {
+      if (r < h) red[r][col] += red[r + h][col];
+      __syncthreads();
+    }
+    if (r == 0 && i < n) put_param(out, pbf, i, red[0][col]);   // (red[0] is these threads' own until the next barrier)
   }
-  if (r == 0 && i < n) put_param(out, pbf, i, red[0][col]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
 inline long long lmin(long long a, long long b) { return a < b ? a : b; }
+
+// A launch holds blocks x threads in 32 bits (more are cut off without an error), so at most 2^21 blocks of up to 1024 threads, a
+// multiple of 8 (xcd_order).  The kernels with a block for each of something stride over more of it; ln_map_fwd, a tile a team, is
+// launched again for the rest
+constexpr int MOST_BLOCKS = 1 << 21;
 
 int check_desc(const RtgLayerNormDesc* d) {
   if (!d) return RTG_ENULL;
@@ -1145,6 +1155,8 @@ Plan plan_bwd(const RtgLayerNormDesc* d) {
   return {LOOPS, (int)(s < 1 ? 1 : lmin(s, 1024))};
 }
 
+dim3 finish_grid(long long n) { return dim3((unsigned)lmin(rtg_ceil_div(n, FIN_COLS), MOST_BLOCKS), 2); }
+
 template <class T>
 int forward(const RtgLayerNormDesc* d, const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, hipStream_t st) {
   const LnShape s = shape_of(d, 1);
@@ -1163,8 +1175,13 @@ int forward(const RtgLayerNormDesc* d, const void* x, const void* w, const void*
   }
 #define LN_MAP_CASE(VEC, ONE, LP, W, CPT)                                                                                    \
   case map_key(LP, W, CPT, ONE):                                                                                             \
-    RTG_KLAUNCH((ln_map_fwd<VEC, LP, W, CPT>), dim3(p.blocks), dim3(map_block(W)), 0, st, s, xt, w, b, yt, mean, rstd);         \
-    return rtg_launch_status();
+    for (int at = 0; at < p.blocks; at += MOST_BLOCKS) {                                                                       \
+      RTG_KLAUNCH((ln_map_fwd<VEC, LP, W, CPT>), dim3((unsigned)lmin(p.blocks - at, MOST_BLOCKS)), dim3(map_block(W)), 0, st, s, xt, w, b, \
+                  yt, mean, rstd, (unsigned)at);                                                                             \
+      const int rc = rtg_launch_status();                                                                                    \
+      if (rc != RTG_OK) return rc;                                                                                           \
+    }                                                                                                                        \
+    return RTG_OK;
   if (is_rows(d)) {
     switch (p.tile) {
       LN_ROW(0) LN_ROW(1) LN_ROW(2) LN_ROW(3) LN_ROW(4) LN_ROW(5) LN_ROW(6) LN_ROW(7) LN_ROW(8) LN_ROW(9)
@@ -1222,7 +1239,7 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
       if (rc != RTG_OK) return rc;
     }
     if (params)
-      RTG_KLAUNCH(ln_row_loop_dw<T>, dim3((unsigned)rtg_ceil_div(d->n, 64 * RtgVec<T>::N), p.blocks), dim3(LOOP_THREADS), 0, st, s, gt, xt, mean,
+      RTG_KLAUNCH(ln_row_loop_dw<T>, dim3((unsigned)lmin(rtg_ceil_div(d->n, 64 * RtgVec<T>::N), MOST_BLOCKS / p.blocks), p.blocks), dim3(LOOP_THREADS), 0, st, s, gt, xt, mean,
                   rstd, part, p.blocks);
   } else if (p.tile != LOOPS) {
     switch (p.tile) {
@@ -1244,7 +1261,7 @@ int backward(const RtgLayerNormDesc* d, const void* dy, const void* x, const flo
 #undef LN_MAP_CASE
   const int rc = rtg_launch_status();
   if (rc != RTG_OK || !params || (is_rows(d) && p.tile >= 0 && p.blocks == 1)) return rc;   // (one block: dw, db are written)
-  RTG_KLAUNCH(ln_finish, dim3((unsigned)rtg_ceil_div(d->n, FIN_COLS), 2), dim3(FIN_COLS * FIN_ROWS), 0, st, (const float*)ws, p.blocks,
+  RTG_KLAUNCH(ln_finish, finish_grid(d->n), dim3(FIN_COLS * FIN_ROWS), 0, st, (const float*)ws, p.blocks,
               d->n, dw, db, s.pbf);
   return rtg_launch_status();
 }
@@ -1274,7 +1291,7 @@ extern "C" int rtg_layernorm_backward(const RtgLayerNormDesc* d, const void* dy,
   const bool params = dweight || dbias;
   if (d->outer == 0 || d->inner == 0) {
     if (!params) return RTG_OK;
-    RTG_KLAUNCH(ln_finish, dim3((unsigned)rtg_ceil_div(d->n, FIN_COLS), 2), dim3(FIN_COLS * FIN_ROWS), 0, (hipStream_t)stream,
+    RTG_KLAUNCH(ln_finish, finish_grid(d->n), dim3(FIN_COLS * FIN_ROWS), 0, (hipStream_t)stream,
                 (const float*)nullptr, 0, d->n, dweight, dbias, d->param_bf16 != 0);
     return rtg_launch_status();
   }
