@@ -94,3 +94,26 @@ def test_rows_longer_than_a_launch_has_threads(n):
     empty = x[:0]
     _, dw, db = ops.layer_norm_backward(empty, empty, mean[:0], rstd[:0])
     assert dw.shape == db.shape == (n,) and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize('sizes', [[2], [5, 3000], [50] * 40, [5_000_003]])
+@pytest.mark.parametrize('scale', [1.0, 1e-3])
+def test_an_update_whose_norm_no_float_holds_is_left_out(sizes, scale):
+    """two finite gradients of 3e38: their norm is 4.2e38, and inf as a float.  What the caller sees as not finite leaves the
+    buffers alone; scaled so that a float holds the norm, it does not"""
+    from test_gradnorm_gpu import state, update
+    s = state(sizes, 1)
+    s['g'][0][:2] = 3e38
+    before = {k: [t.clone() for t in s[k]] for k in s}
+    norm = update(s, 0.05, grad_scale=scale)
+    assert torch.isinf(norm) == (scale == 1.0)
+    for k in 'pmvt':
+        assert all(torch.equal(a, b) for a, b in zip(s[k], before[k])) == (scale == 1.0), k
+
+
+def test_clipping_by_a_norm_no_float_holds():
+    """the returned norm is inf, the factor that of the norm itself"""
+    from rtg import ops
+    t = torch.full((4,), 3e38, device=DEV)                      # 6e38
+    assert torch.isinf(ops.clip_grads_([t], 60.0)) and torch.isinf(ops.total_norm([torch.full((4,), 3e38, device=DEV)]))
+    assert ((t - 30.0).abs() <= 30.0 * 2.0 ** -22).all()        # (3e38 as a float, the factor, the product: half a step each)

@@ -85,7 +85,7 @@ __device__ __forceinline__ double all_partials(const double* __restrict__ part, 
 template <int KIND>
 __device__ __forceinline__ double norm_of(double joined) { return KIND == RTG_NORM_L2 ? sqrt(joined) : joined; }
 
-// min(1, max_norm / (norm + 1e-6)): 0 for an infinite norm, NaN for a NaN
+// min(1, max_norm / (norm + 1e-6)) of the norm in 64 bits: 0 for an infinite norm, NaN for a NaN
 __device__ __forceinline__ float clip_factor(double norm, double max_norm) {
   const double f = max_norm / (norm + 1e-6);
   return f < 1.0 || f != f ? (float)f : 1.f;
@@ -230,7 +230,7 @@ __device__ __forceinline__ AdamScalars adam_scalars(double norm, float step, boo
   s.step_size = (float)(r.lr / (1.0 - pow(r.b1, t)));
   s.bc2s = (float)sqrt(1.0 - pow(r.b2, t));
   s.scale = r.gscale * clip_factor(norm, r.max_norm);
-  s.go = isfinite(norm) && !flagged ? 1.f : 0.f;
+  s.go = isfinite((float)norm) && !flagged ? 1.f : 0.f;   // (the norm as the caller sees it)
   return s;
 }
 __device__ __forceinline__ bool adam_flagged(const float* flag) { return flag && isnan(*flag); }

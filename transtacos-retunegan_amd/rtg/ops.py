@@ -1643,7 +1643,8 @@ def clip_grads_(grads, max_norm, norm_type=2.0):
     """Scale a list of gradients in place by min(1, max_norm / (norm + 1e-6)) -> their norm before (a float32 device scalar):
     what torch.nn.utils.clip_grad_norm_ does to the .grad of its parameters (train.clip_grad_norm_ takes parameters), on the
     device alone.  A norm within the limit costs one read of the gradients and no write.  An infinite norm scales by 0, a
-    NaN by NaN, as torch's does."""
+    NaN by NaN, as torch's does; of finite gradients whose norm no float holds (it is returned as inf) the factor is that of the
+    norm in 64 bits."""
     kind, limit = _norm_kind(norm_type), _limit(max_norm)
     g = _GradList('clip_grads_', grads, True)
     ws, out = g.ws(), torch.empty((), device=g.device)
@@ -1659,7 +1660,7 @@ def clipped_adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, max_norm, lr=1e-
     clipped to max_norm over ALL of them -> the norm of grads * grad_scale before (`out`, or a new device scalar).  The factor
     is applied where the update reads the gradients: they keep their values and are not written.  steps: one float32 device
     scalar per buffer, advanced by the call; loss_flags: None, or per buffer a device scalar (or None) whose NaN leaves that
-    buffer, its moments and its step alone.  A norm that is not finite leaves all of them alone."""
+    buffer, its moments and its step alone.  A norm that is not finite (as it is returned: in a float) leaves all of them alone."""
     limit = _limit(max_norm)
     cols = [list(c) for c in (params, grads, exp_avgs, exp_avg_sqs, steps)]
     n = len(cols[0])
