@@ -115,3 +115,35 @@ def test_an_import_leaves_the_threads_of_autograd_alone():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     out = subprocess.run([sys.executable, '-c', code], cwd=root, env=env, capture_output=True, text=True, check=True)
     assert out.stdout.split()[-2:] == ['True', 'True']
+
+
+@pytest.mark.parametrize('name', ['Generator_RefineGAN_small', 'Generator_RefineGAN'])
+def test_generators_list_their_layer_norms(name):
+    """a layer norm added to a generator joins its flat buffers, beside the parameter that the generator lists itself"""
+    from models import generator
+    from models.layers import LayerNorm
+
+    class Normed(getattr(generator, name)):
+        def __init__(self):
+            super().__init__()
+            self.norm = LayerNorm(32)
+    own = [n for n, _ in getattr(generator, name)()._bank_params()]
+    net = Normed()
+    assert own == ['noise.w']
+    got = dict(net._bank_params())
+    assert set(got) == {'norm.weight', 'norm.bias', 'noise.w'} and got['norm.weight'] is net.norm.weight and got['noise.w'] is net.noise.w
+
+
+def test_a_layer_norm_left_out_of_the_bank_is_refused():
+    from models.layers import BankedModel, LayerNorm
+    from rtg.lib import RtgError
+
+    class Net(BankedModel):
+        def __init__(self):
+            super().__init__()
+            self.norm, self.scale = LayerNorm(4), torch.nn.Parameter(torch.ones(3))
+
+        def _extra_bank_params(self):
+            return [('scale', self.scale), ('norm.weight', self.norm.weight)]
+    with pytest.raises(RtgError, match='norm.bias'):
+        Net()._bank_params()

@@ -183,7 +183,7 @@ class Generator_RefineGAN_small(BankedModel):
         self._wn_removed = False
 
     def _extra_bank_params(self):
-        return [('noise.w', self.noise.w)]
+        return [*super()._extra_bank_params(), ('noise.w', self.noise.w)]
 
     def forward(self, x, y, noise_list=None):
         """noise_list: optional six pre-drawn U[0,1) tensors (parity tests); by default drawn on the device."""
@@ -244,7 +244,7 @@ class Generator_RefineGAN(BankedModel):
         self._wn_removed = False
 
     def _extra_bank_params(self):
-        return [('noise.w', self.noise.w)]
+        return [*super()._extra_bank_params(), ('noise.w', self.noise.w)]
 
     def forward(self, x, y, noise_list=None):
         tok = self.token()

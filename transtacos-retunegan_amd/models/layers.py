@@ -93,6 +93,15 @@ class BankedModel(nn.Module):
         appends its own to this list)"""
         return [(f'{n}.{k}', p) for n, m in self.named_modules() if isinstance(m, LayerNorm) for k, p in m.named_parameters()]
 
+    def _bank_params(self):
+        """_extra_bank_params, which a model may have overridden: a layer norm that it leaves out would never be updated"""
+        extra = self._extra_bank_params()
+        for n, p in BankedModel._extra_bank_params(self):
+            if not any(p is q for _, q in extra):
+                raise RtgError(f'{type(self).__name__}: {n} is missing from _extra_bank_params (an override adds its own parameters to '
+                               'super()._extra_bank_params())')
+        return extra
+
     def _apply(self, fn, *a, **k):
         r = super()._apply(fn, *a, **k)
         self._bank = None           # .to()/.cuda()/.float() re-materialise the parameters: rebuild the flat views
@@ -111,7 +120,7 @@ class BankedModel(nn.Module):
                            'per GPU; train.Trainer does it for its `dev`)')
         if self._bank is None or self._bank.device != dev or not self._bank.check_views():
             layers = [(n, m) for n, m in self.named_modules() if isinstance(m, WNConv)]
-            self._bank = WeightBank(layers, self._extra_bank_params(), dev)
+            self._bank = WeightBank(layers, self._bank_params(), dev)
             self._bank.wgrad_side = bool(getattr(self, 'wgrad_side', False))
             for ly in self._bank.layers:
                 ly.module._layer = ly
