@@ -509,7 +509,7 @@ int rtg_layernorm_backward(const RtgLayerNormDesc* d, const void* dy, const void
  *   rtg_adamw_clipped   the update of rtg_adamw for n flat buffers with gradients read as g * grad_scale * factor, the
  *                  factor that of rtg_grad_clip over all n with norm * grad_scale, the 2-norm (the gradients stay as they
  *                  are).  A buffer whose *loss_flag is NaN is left alone, its step counter included; with a *norm_out
- *                  that is not finite every buffer is.
+ *                  that is not finite every buffer is.  Nothing that is written may overlap anything else, a loss flag included.
  * ws: rtg_grad_ws(n) doubles of scratch.
  * ------------------------------------------------------------------------------------------------------------ */
 enum { RTG_NORM_L2 = 0, RTG_NORM_MAX = 1 };

@@ -147,3 +147,19 @@ def test_a_layer_norm_left_out_of_the_bank_is_refused():
             return [('scale', self.scale), ('norm.weight', self.norm.weight)]
     with pytest.raises(RtgError, match='norm.bias'):
         Net()._bank_params()
+
+
+def test_a_loss_flag_inside_a_written_buffer_is_refused():
+    """flags are read while, or after, other buffers are written: what the update itself writes is none"""
+    import ctypes as C
+    from rtg.lib import AdamWJob, lib
+    one = C.c_void_p(256)
+
+    def adamw(*jobs, out=one):
+        return lib.rtg_adamw_clipped(len(jobs), (AdamWJob * len(jobs))(*jobs), 1.0, 1e-3, 0.9, 0.99, 1e-8, 0.01, 1.0, one, out, None)
+    # parameters, gradients, moments, step, flag, elements
+    first, second = [512, 1024, 1536, 2048, 2560, None, 10], [8512, 81024, 81536, 82048, 82560, None, 10]
+    for flag in (512, 548, 1536, 2048 + 36, 2560, 256, 2558):
+        assert adamw(tuple(first[:5] + [flag, 10])) == -1, flag
+        assert adamw(tuple(first), tuple(second[:5] + [flag, 10])) == -1, flag
+        assert adamw(tuple(first[:5] + [1024, 10]), tuple(second[:5] + [flag, 10]), out=one) == -1, flag

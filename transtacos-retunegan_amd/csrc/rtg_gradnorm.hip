@@ -393,7 +393,7 @@ int check_list(int n, void* const* grads, const long long* counts, const int* bf
   return RTG_OK;
 }
 
-struct Range { uintptr_t lo, hi; };
+struct Range { uintptr_t lo, hi; bool written; };
 // no two ranges share a byte: workgroups of one launch would write what others read.  A list in the order of its addresses
 // (the views of a flat buffer) needs no sorting.
 int disjoint(Range* r, long long n) {
@@ -405,6 +405,20 @@ int disjoint(Range* r, long long n) {
   if (ordered()) return RTG_OK;
   std::sort(r, r + n, [](const Range& a, const Range& b) { return a.lo < b.lo; });
   return ordered() ? RTG_OK : RTG_EINVAL;
+}
+
+// the float at p shares a byte with a range that is written (r: disjoint, so in the order of the addresses)
+bool is_written(const Range* r, long long n, const float* p) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+  for (const Range* q = std::upper_bound(r, r + n, lo + 3, [](uintptr_t at, const Range& a) { return at < a.lo; }); q > r;) {
+    --q;
+    if (q->hi > lo) {
+      if (q->written) return true;
+    } else if (q->hi > q->lo) {
+      break;                                               // (empty ranges are passed over)
+    }
+  }
+  return false;
 }
 
 template <int KIND>
@@ -479,7 +493,7 @@ extern "C" int rtg_grad_clip(int n, void* const* grads, const long long* counts,
     int k = 0;
     for (int i = 0; i < n; ++i) {
       const uintptr_t lo = reinterpret_cast<uintptr_t>(grads[i]);
-      if (counts[i] > 0) r[k++] = Range{lo, lo + (uintptr_t)counts[i] * (bf16[i] ? 2 : 4)};
+      if (counts[i] > 0) r[k++] = Range{lo, lo + (uintptr_t)counts[i] * (bf16[i] ? 2 : 4), true};
     }
     const int apart = disjoint(r.get(), k);
     if (apart != RTG_OK) return apart;
@@ -506,16 +520,23 @@ extern "C" int rtg_adamw_clipped(int n, const RtgAdamWJob* jobs, double max_norm
     if (!r) return RTG_ERANGE;
     for (int i = 0; i < n; ++i) {
       const RtgAdamWJob& j = jobs[i];
-      const void* p[5] = {j.params, j.grads, j.exp_avg, j.exp_avg_sq, j.step_state};
+      const void* p[5] = {j.params, j.exp_avg, j.exp_avg_sq, j.step_state, j.grads};
       for (int k = 0; k < 5; ++k) {
         const uintptr_t lo = reinterpret_cast<uintptr_t>(p[k]);
-        r[5 * (size_t)i + k] = Range{lo, lo + (k < 4 ? 4 * (uintptr_t)j.n : 4)};
+        r[5 * (size_t)i + k] = Range{lo, lo + (k != 3 ? 4 * (uintptr_t)j.n : 4), k < 4};
       }
     }
     const uintptr_t out = reinterpret_cast<uintptr_t>(norm_out);
-    r[5 * (size_t)n] = Range{out, out + (out ? 4 : 0)};
+    r[5 * (size_t)n] = Range{out, out + (out ? 4 : 0), true};
     const int apart = disjoint(r.get(), 5ll * n + 1);
     if (apart != RTG_OK) return apart;
+    // (the flags of later buffers are read when earlier ones have been updated)
+    const float* last = nullptr;
+    for (int i = 0; i < n; ++i) {
+      const float* flag = jobs[i].loss_flag;
+      if (flag && flag != last && is_written(r.get(), 5ll * n + 1, flag)) return RTG_EINVAL;
+      last = flag;
+    }
   }
   hipStream_t st = (hipStream_t)stream;
   const AdamRates rates{max_norm, lr, beta1, beta2, grad_scale};

@@ -1689,7 +1689,7 @@ def clipped_adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, max_norm, lr=1e-
     ws = torch.empty(lib.rtg_grad_ws(n), device=dev, dtype=torch.float64)
     check(timed_bw('adamw_clipped', 32 * sum(p.numel() for p in cols[0]), lambda: lib.rtg_adamw_clipped(
         n, jobs, limit, lr, betas[0], betas[1], eps, weight_decay, grad_scale, ws.data_ptr(), out.data_ptr(), _stream())),
-          'adamw_clipped (do buffers overlap?)')
+          'adamw_clipped (do buffers overlap, or is a loss flag one that the update writes?)')
     torch.autograd.graph.increment_version(cols[0] + cols[2] + cols[3] + cols[4])
     return out
 
