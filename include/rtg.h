@@ -505,7 +505,7 @@ int rtg_layernorm_backward(const RtgLayerNormDesc* d, const void* dy, const void
  *   rtg_grad_clip  ... and g *= min(1, max_norm / (norm + 1e-6)); nothing is written where that factor is 1 (an infinite
  *                  norm: factor 0; a NaN: NaN).  Finite gradients whose norm no float holds are scaled too (the factor comes from
  *                  the 64-bit norm and is a float: below 1.2e-38 it has fewer bits), *norm_out is infinite then.  Tensors must
- *                  not overlap.
+ *                  not overlap, nor hold norm_out.
  *   rtg_adamw_clipped   the update of rtg_adamw for n flat buffers with gradients read as g * grad_scale * factor, the
  *                  factor that of rtg_grad_clip over all n with norm * grad_scale, the 2-norm (the gradients stay as they
  *                  are).  A buffer whose *loss_flag is NaN is left alone, its step counter included; with a *norm_out

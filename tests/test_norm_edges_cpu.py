@@ -163,3 +163,11 @@ def test_a_loss_flag_inside_a_written_buffer_is_refused():
         assert adamw(tuple(first[:5] + [flag, 10])) == -1, flag
         assert adamw(tuple(first), tuple(second[:5] + [flag, 10])) == -1, flag
         assert adamw(tuple(first[:5] + [1024, 10]), tuple(second[:5] + [flag, 10]), out=one) == -1, flag
+
+
+def test_a_norm_inside_a_clipped_gradient_is_refused():
+    import ctypes as C
+    from rtg.lib import lib
+    ptrs, counts, bf16 = (C.c_void_p * 2)(4096, 512), (C.c_longlong * 2)(10, 10), (C.c_int * 2)(0, 1)
+    for out in (4096, 4132, 512, 516, 528):
+        assert lib.rtg_grad_clip(2, ptrs, counts, bf16, 0, 1.0, C.c_void_p(64), C.c_void_p(out), None) == -1, out

@@ -497,6 +497,7 @@ extern "C" int rtg_grad_clip(int n, void* const* grads, const long long* counts,
     }
     const int apart = disjoint(r.get(), k);
     if (apart != RTG_OK) return apart;
+    if (is_written(r.get(), k, norm_out)) return RTG_EINVAL;
   }
   return kind == RTG_NORM_L2 ? clip<RTG_NORM_L2>(n, grads, counts, bf16, max_norm, ws, norm_out, (hipStream_t)stream)
                              : clip<RTG_NORM_MAX>(n, grads, counts, bf16, max_norm, ws, norm_out, (hipStream_t)stream);
