@@ -332,7 +332,7 @@ __global__ __launch_bounds__(BLK) void ln_row_bwd(LnShape s, const T* __restrict
 // Feature maps.  A wave holds a tile of LP * N adjacent positions (N in a lane's vector) with its 64 / LP channel lanes times
 // CPT channels each in registers; W waves share the channels of a tile where one cannot hold them.  Every load is a whole
 // 16 * LP bytes of a channel's row, CPT of them in flight per lane: (32, 128, 2048) floats 12.0 us forward (5.6 TB/s), 24 backward;
-// (16, 512, 1025), whose channels start anywhere in a line, 14.6 and 31.5.
+// (16, 512, 1025), whose channels start anywhere in a line, 13.7 and 28.8 with the join of dw and db.
 // ---------------------------------------------------------------------------------------------------------------------
 // workgroup b of a grid of 8 k runs on XCD b % 8 (each has its own L2): neighbours in the order of the tiles are put on one XCD, so
 // a line that two tiles share — rows of a map that do not start on a line — is fetched once
@@ -596,7 +596,8 @@ __global__ __launch_bounds__(map_block(W)) void ln_map_bwd(LnShape s, const T* _
 // ---------------------------------------------------------------------------------------------------------------------
 // Kernels for any size.  A row or a column of channels that no register kernel holds is read once per sum (the later reads
 // come from L2 or the memory-side cache): 1000 rows of 40000 floats 97 us forward, 194 backward (3.3 and 2.5 TB/s of what has to
-// move).  They also serve rows of less than a vector, a thread each (1000000 x 5 floats 20 and 46 us).
+// move).  ln_tiny serves rows of less than a vector, a thread each (1000000 x 3 floats 8.9 and 14.1 us, 1000000 x 7 bf16 values
+// 14.9 and 24.6, and 4 for the join: 2.4 .. 3.6 and 2.0 .. 3.1 TB/s of what has to move).
 // ---------------------------------------------------------------------------------------------------------------------
 template <int BLK>
 __device__ __forceinline__ float loop_sum(float v, float* red) {
@@ -754,7 +755,7 @@ __global__ __launch_bounds__(LOOP_THREADS) void ln_row_loop_dw(LnShape s, const 
   }
 }
 
-// rows of less than a vector (n < 8): a thread a row
+// rows of less than a vector (fewer than 4 floats, than 8 bf16 values): a thread a row
 constexpr int TINY_THREADS = 256, TINY_MOST = 7;
 template <class T>
 __global__ __launch_bounds__(TINY_THREADS) void ln_tiny_fwd(LnShape s, const T* __restrict__ x, const void* __restrict__ w,
@@ -1011,8 +1012,10 @@ constexpr int LOOPS = -1, TINY = -2;
 // Rows: threads per row, 16-byte vectors per thread, threads per block.  Over 13 widths from 64 to 16384 and row counts from 1 to
 // 65536 these tiles are within 5 % of the best of 20 (forward) and 40 (backward); what they weigh: a wave's rows need no
 // barrier (up to two vectors a thread), a block's row two; the backward holds sixteen elements a thread at most (the weight, dw
-// and db take a register each).  Forward, as many blocks as fit up to 64 MB of rows (8192 x 2048 bf16 14.2 us, with half of them
-// 15.6; 4096 x 1024 floats 7.8 and 8.5; not of 1024 threads: 2048 x 16384 bf16 28.7 and 26.9), half of them beyond: each walks its
+// and db take a register each).  The shortest rows have eight lanes whatever their length: of five floats two are busy (1000000
+// rows of them 18.8 us forward, 35.6 backward).  Forward, as many blocks as fit up to 64 MB of rows (8192 x 2048 bf16, side by
+// side, 14.2 us, with half of them 15.6, and 13.6 .. 16.0 from program to program; 4096 x 1024 floats 7.8 and 8.5; not of 1024
+// threads: 2048 x 16384 bf16 28.7 and 26.9), half of them beyond: each walks its
 // rows with the next in flight, and fewer rows of HBM are open at a time (65536 x 1024 floats 81 us, with all of them 83, with a
 // quarter 110; 16384 x 4096 bf16 45.8, 48.6, 50.2).
 struct RowTile { int tpr, vpt, blk; };
