@@ -117,3 +117,87 @@ def test_clipping_by_a_norm_no_float_holds():
     t = torch.full((4,), 3e38, device=DEV)                      # 6e38
     assert torch.isinf(ops.clip_grads_([t], 60.0)) and torch.isinf(ops.total_norm([torch.full((4,), 3e38, device=DEV)]))
     assert ((t - 30.0).abs() <= 30.0 * 2.0 ** -22).all()        # (3e38 as a float, the factor, the product: half a step each)
+
+
+@pytest.mark.parametrize('shape,dim', [((300, 1024), -1), ((3, 64, 200), 1)])
+def test_training_passes_captured_into_graphs(shape, dim):
+    """forward and backward through autograd in two graphs, replayed in turn with new inputs and eager passes between"""
+    from rtg import ops
+    w, b = params(shape[dim], torch.float32, 1)
+
+    def both(x, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = ops.layer_norm(*leaves, dim=dim)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    ins = [(make(shape, torch.float32, s), make(shape, torch.float32, s + 1, 0.0)) for s in (10, 20)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(*ins[0])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for x, dy in ins:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = both(x, dy)
+        graphs.append((g, out))
+    for r in range(3):
+        for k, ((g, out), (x, dy)) in enumerate(zip(graphs, ins)):
+            x.copy_(make(shape, torch.float32, 100 * r + k))
+            dy.copy_(make(shape, torch.float32, 100 * r + k + 50, 0.0))
+            g.replay()
+            want = both(x, dy)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(out, want)), (r, k)
+
+
+def test_training_passes_of_two_threads_and_streams():
+    """two threads, each with a stream and layouts of its own, while nobody waits for the other"""
+    import threading
+    from rtg import ops
+    work = []
+    for k, (shape, dim, cut) in enumerate((((6, 48, 300), 1, lambda t: t[:, :, 5:270]), ((500, 1100), -1, lambda t: t[:, 3:1003]))):
+        x = cut(make(shape, torch.float32, k))
+        work.append((x, *params(x.shape[dim], torch.float32, k), make(tuple(x.shape), torch.float32, k + 5, 0.0), dim))
+
+    def one(x, w, b, dy, dim):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = ops.layer_norm(*leaves, dim=dim)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    want = [one(*w) for w in work]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def run(k):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    got[k].append(one(*work[k]))
+            st.synchronize()
+        except Exception as e:                                  # (shown below: a thread's exception is not the test's)
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed, failed
+    assert all(len(g) == 20 and all(torch.equal(a, c) for out in g for a, c in zip(out, want[k])) for k, g in enumerate(got))
+
+
+def test_a_map_of_more_positions_than_a_tile_counts():
+    """2^24 positions and more: the kernels for any size"""
+    from rtg import ops
+    shape = (1, 5, (1 << 24) + 70)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x, dy = (torch.empty(shape, device=DEV, dtype=torch.bfloat16).normal_(m, 1.0, generator=gen) for m in (1.0, 0.0))
+    w, b = params(5, torch.float32, 2)
+    y, mean, rstd = ops.layer_norm_forward(x, w, b, dim=1, keep=True)
+    dx, _, _ = ops.layer_norm_backward(dy, x, mean, rstd, w, dim=1)
+    ref = Reference(x, w, b, 1e-5).backward(dy, torch.float32)
+    inside(y, ref.y, ref.y_off, 'y')
+    inside(dx, ref.dx, ref.dx_off, 'dx')
+    ones, zeros = torch.ones(shape[2], device=DEV), torch.zeros(shape[2], device=DEV)      # (sums of whole numbers: exact)
+    x, dy = (torch.randint(-1, 2, shape, generator=gen, device=DEV).bfloat16() for _ in range(2))
+    _, dw, db = ops.layer_norm_backward(dy, x, zeros, ones, w, dim=1)
+    assert torch.equal(dw.double(), (dy.double() * x.double()).sum((0, 2))) and torch.equal(db.double(), dy.double().sum((0, 2)))
